@@ -8,7 +8,7 @@ import os
 _PKG_DIR = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_PKG_DIR, "libasuka_b200.so")
 
-F16, BF16, F32, I32, U8 = 0, 1, 2, 3, 4
+F16, BF16, F32, I32, U8, I8, E4M3 = 0, 1, 2, 3, 4, 5, 6
 
 SCORE_SUM, SCORE_SUM_SQ, SCORE_PERTURBED, SCORE_CORM = 0, 1, 2, 3
 SELECT_TOPK, SELECT_TOPK_RECENT, SELECT_ROCO = 0, 1, 2
@@ -68,6 +68,24 @@ class GatherParams(ctypes.Structure):
   _fields_ = [("k", Tensor), ("v", Tensor), ("idx", Tensor), ("k_out", Tensor), ("v_out", Tensor)]
 
 
+class KvCache(ctypes.Structure):
+  _fields_ = [("k", Tensor), ("v", Tensor), ("k_scale", Tensor), ("v_scale", Tensor)]
+
+
+class QuantKvParams(ctypes.Structure):
+  _fields_ = [("k", Tensor), ("v", Tensor), ("idx", Tensor), ("start", Tensor), ("count", Tensor), ("cache", KvCache)]
+
+
+class DequantKvParams(ctypes.Structure):
+  _fields_ = [("cache", KvCache), ("idx", Tensor), ("len", Tensor), ("k_out", Tensor), ("v_out", Tensor)]
+
+
+class AttnCacheParams(ctypes.Structure):
+  _fields_ = [("q", Tensor), ("out", Tensor), ("lse", Tensor), ("cache", KvCache), ("len", Tensor), ("prefix", KvCache),
+              ("prefix_len", Tensor), ("softmax_scale", ctypes.c_float), ("causal", ctypes.c_int32),
+              ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_uint64)]
+
+
 class CaseParams(ctypes.Structure):
   _fields_ = [("q", Tensor), ("k", Tensor), ("v", Tensor), ("out", Tensor), ("score", Tensor),
               ("score_sq", Tensor), ("exp_rand", Tensor), ("idx", Tensor),
@@ -97,6 +115,10 @@ SYMBOLS = {
     "asuka_b200_select_topk": (ctypes.c_int, [ctypes.POINTER(SelectParams), ctypes.c_void_p]),
     "asuka_b200_pool_scores": (ctypes.c_int, [ctypes.POINTER(Tensor), ctypes.POINTER(Tensor), ctypes.c_int32, ctypes.c_void_p]),
     "asuka_b200_gather_kv": (ctypes.c_int, [ctypes.POINTER(GatherParams), ctypes.c_void_p]),
+    "asuka_b200_quant_kv": (ctypes.c_int, [ctypes.POINTER(QuantKvParams), ctypes.c_void_p]),
+    "asuka_b200_dequant_kv": (ctypes.c_int, [ctypes.POINTER(DequantKvParams), ctypes.c_void_p]),
+    "asuka_b200_attn_cache": (ctypes.c_int, [ctypes.POINTER(AttnCacheParams), ctypes.c_void_p]),
+    "asuka_b200_attn_cache_workspace_bytes": (ctypes.c_int, [ctypes.POINTER(AttnCacheParams), ctypes.POINTER(ctypes.c_size_t)]),
     "asuka_b200_sima_workspace_bytes": (ctypes.c_int, [ctypes.POINTER(SimaParams), ctypes.POINTER(ctypes.c_size_t)]),
     "asuka_b200_sima_fwd": (ctypes.c_int, [ctypes.POINTER(SimaParams), ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p]),
     "asuka_b200_ea_fwd": (ctypes.c_int, [ctypes.POINTER(SimaParams), ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p]),

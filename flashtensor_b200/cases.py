@@ -14,6 +14,7 @@ the scores): they return the kept key indices as ascending int32.
 import torch
 
 from . import ops
+from .cache import KVCache
 
 
 class _Case:
@@ -33,7 +34,7 @@ class _Case:
     # scripts (cases/attn.py, cases/attn_h2o.py) run grouped-query attention, supported here by
     # the classes that set `allow_gqa`
     assert self.head_num % self.kv_head_num == 0
-    assert self.group_size == 1 or self.allow_gqa, "grouped-query attention: Attn, Gemma2, H2O only"
+    assert self.group_size == 1 or self.allow_gqa, "grouped-query attention: Attn, Gemma2, H2O, CacheAttn, PrefixAttn only"
 
   def __call__(self, *args, **kwargs):
     return self.forward(*args, **kwargs)
@@ -267,6 +268,55 @@ class EA(SimA):
 
   def prepare(self, batch_size=8, q_len=8192, kv_len=None, dtype=torch.float16, device=None):
     return _Case.prepare(self, batch_size, q_len, q_len, dtype, device)
+
+
+class CacheAttn(_Case):
+  """Attention of new tokens over a ``KVCache`` of ragged sequences, 16 or 8 bits (no counterpart in the
+  reference, whose cases end with the prefill): a generation's step behind ``Attn`` or ``H2O.select``."""
+  allow_gqa = True
+
+  def __init__(self, kv_head_num=32, head_num=32, head_dim=128, causal=True):
+    super().__init__(kv_head_num, head_num, head_dim)
+    self.causal = causal
+
+  def _check(self, q, *caches):
+    super()._check(q)
+    for c in caches:
+      if c.k.dim() == 4 and c.k.size(2) != self.kv_head_num:
+        raise RuntimeError(f"expected {self.kv_head_num} key/value heads, got {c.k.shape[2]}")
+
+  def forward(self, q, cache, kv_len=None):
+    self._check(q, cache)
+    return ops.attn_cache(q, cache, kv_len, causal=self.causal)
+
+  def prepare(self, batch_size=1, q_len=1, kv_len=4096, dtype=torch.float16, device=None):
+    """As the other cases' ``prepare``, the keys and values in a 16-bit cache."""
+    ins = super().prepare(batch_size, q_len, kv_len, dtype, device)["input"]
+    return {"input": {"q": ins["q"], "cache": KVCache(ins["k"], ins["v"])}, "output": list(self.output_names)}
+
+  def get_mem_size(self, batch_size=1, q_len=1, kv_len=4096):
+    return 2 * batch_size * self.head_dim * (q_len * self.head_num + kv_len * self.kv_head_num)
+
+
+class PrefixAttn(CacheAttn):
+  """``CacheAttn`` for sequences that share a prefix: ``prefix`` is a ``KVCache`` of G sequences, each seen by
+  B / G consecutive sequences of q ahead of their own rows in ``cache``, and read once for all of them."""
+
+  def forward(self, q, prefix, cache, kv_len=None, prefix_len=None):
+    self._check(q, prefix, cache)
+    return ops.attn_prefix(q, prefix, cache, kv_len, prefix_len, causal=self.causal)
+
+  def prepare(self, batch_size=1, q_len=1, kv_len=4096, dtype=torch.float16, device=None):
+    """One prefix of `kv_len` rows, and `q_len` rows of each sequence's own."""
+    ins = CacheAttn.prepare(self, batch_size, q_len, q_len, dtype, device)["input"]
+    shared = CacheAttn.prepare(self, 1, q_len, kv_len, dtype, device)["input"]["cache"]
+    return {"input": {"q": ins["q"], "prefix": shared, "cache": ins["cache"]}, "output": list(self.output_names)}
+
+  def get_flops(self, batch_size=1, q_len=1, kv_len=4096):
+    return super().get_flops(batch_size, q_len, kv_len + q_len)
+
+  def get_mem_size(self, batch_size=1, q_len=1, kv_len=4096):
+    return super().get_mem_size(batch_size, q_len, q_len) + 2 * self.head_dim * kv_len * self.kv_head_num
 
 
 CASES = {"EA": EA, "Attn": Attn, "Gemma2": Gemma2, "SnapKV": SnapKV, "Corm": Corm, "H2O": H2O, "KeyFormer": KeyFormer, "RoCo": RoCo, "SimA": SimA}

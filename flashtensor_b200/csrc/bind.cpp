@@ -9,6 +9,7 @@
 #include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
+#include <torch/csrc/Dtype.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
@@ -71,6 +72,8 @@ asuka_tensor desc(const at::Tensor& t) {
     case at::kInt: d.dtype = ASUKA_I32; break;
     case at::kByte:
     case at::kBool: d.dtype = ASUKA_U8; break;
+    case at::kChar: d.dtype = ASUKA_I8; break;
+    case at::kFloat8_e4m3fn: d.dtype = ASUKA_E4M3; break;
     default:
       PyErr_Format(PyExc_TypeError, "unsupported dtype %s", c10::toString(t.scalar_type()));
       throw BadArg();
@@ -466,6 +469,118 @@ PyObject* gather_kv(PyObject*, PyObject* const* a, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// a[0..3]: k, v, k_scale, v_scale (None for 16 bits)
+struct Cache {
+  at::Tensor k, v, k_scale, v_scale;
+  explicit Cache(PyObject* const* a)
+      : k(optional_tensor(a[0])), v(optional_tensor(a[1])), k_scale(optional_tensor(a[2])), v_scale(optional_tensor(a[3])) {}
+  asuka_kv_cache c() const { return asuka_kv_cache{desc(k), desc(v), desc(k_scale), desc(v_scale)}; }
+};
+
+// (k, v, cache's k, v, k_scale, v_scale, start, count, idx) -> None
+PyObject* quant_kv(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  try {
+    want_args(n, 9);
+    const at::Tensor &k = tensor_arg(a[0]), &v = tensor_arg(a[1]);
+    const Cache cache(a + 2);
+    const at::Tensor start = optional_tensor(a[6]), count = optional_tensor(a[7]), idx = optional_tensor(a[8]);
+    OnDevice on({&k, &v, &cache.k, &cache.v, &cache.k_scale, &cache.v_scale, &start, &count, &idx});
+    asuka_quant_kv_params p;
+    p.k = desc(k);
+    p.v = desc(v);
+    p.idx = desc(idx);
+    p.start = desc(start);
+    p.count = desc(count);
+    p.cache = cache.c();
+    call("asuka_b200_quant_kv", [&] { return asuka_b200_quant_kv(&p, on.stream); });
+    Py_RETURN_NONE;
+  } catch (const BadArg&) {
+    return nullptr;
+  }
+  END_HANDLE_TH_ERRORS
+}
+
+// (cache's k, v, k_scale, v_scale, dtype, idx, len, length (-1: all)) -> (k rows, v rows)
+PyObject* dequant_kv(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  try {
+    want_args(n, 8);
+    tensor_arg(a[0]);
+    const Cache cache(a);
+    if (!THPDtype_Check(a[4])) {
+      PyErr_SetString(PyExc_TypeError, "expected a torch.dtype");
+      throw BadArg();
+    }
+    const at::ScalarType dtype = reinterpret_cast<THPDtype*>(a[4])->scalar_type;
+    const at::Tensor idx = optional_tensor(a[5]), len = optional_tensor(a[6]);
+    const int64_t length = static_cast<int64_t>(int_arg(a[7]));
+    OnDevice on({&cache.k, &cache.v, &cache.k_scale, &cache.v_scale, &idx, &len});
+    if (cache.k.dim() != 4 || (idx.defined() && idx.dim() != 3)) call("asuka_b200_dequant_kv", [] { return ASUKA_ERR_BAD_SHAPE; });
+    if (length < -1 || (idx.defined() && length >= 0)) call("asuka_b200_dequant_kv", [] { return ASUKA_ERR_BAD_ARGUMENT; });
+    const int64_t rows = idx.defined() ? idx.size(2) : length >= 0 ? length : cache.k.size(1);
+    const at::Tensor ko = empty({cache.k.size(0), rows, cache.k.size(2), cache.k.size(3)}, dtype, cache.k);
+    const at::Tensor vo = empty(ko.sizes(), dtype, cache.k);
+    asuka_dequant_kv_params p;
+    p.cache = cache.c();
+    p.idx = desc(idx);
+    p.len = desc(len);
+    p.k_out = desc(ko);
+    p.v_out = desc(vo);
+    call("asuka_b200_dequant_kv", [&] { return asuka_b200_dequant_kv(&p, on.stream); });
+    return tuple({wrap(ko), wrap(vo)});
+  } catch (const BadArg&) {
+    return nullptr;
+  }
+  END_HANDLE_TH_ERRORS
+}
+
+// (q, cache's k, v, k_scale, v_scale, len, prefix's k, v, k_scale, v_scale, prefix_len, causal, softmax_scale, return_lse, out)
+//   -> out | (out, lse)
+PyObject* attn_cache(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  try {
+    want_args(n, 15);
+    const at::Tensor& q0 = tensor_arg(a[0]);
+    const at::Tensor q = as4d(q0);
+    tensor_arg(a[1]);
+    const Cache cache(a + 1), prefix(a + 6);
+    const at::Tensor len = optional_tensor(a[5]), prefix_len = optional_tensor(a[10]);
+    at::Tensor out = optional_tensor(a[14]), lse;
+    OnDevice on({&q, &cache.k, &cache.v, &cache.k_scale, &cache.v_scale, &len, &prefix.k, &prefix.v, &prefix.k_scale,
+                 &prefix.v_scale, &prefix_len, &out});
+    if (q.dim() != 4) call("asuka_b200_attn_cache", [] { return ASUKA_ERR_BAD_SHAPE; });
+    if (!out.defined()) out = empty(q.sizes(), q.scalar_type(), q);
+    const bool want_lse = bool_arg(a[13]);
+    if (want_lse) lse = empty({q.size(0), q.size(2), q.size(1)}, at::kFloat, q);
+    asuka_attn_cache_params p;
+    std::memset(&p, 0, sizeof(p));
+    p.q = desc(q);
+    p.out = desc(as4d(out));
+    p.lse = desc(lse);
+    p.cache = cache.c();
+    p.len = desc(len);
+    p.prefix = prefix.c();
+    p.prefix_len = desc(prefix_len);
+    p.softmax_scale = static_cast<float>(float_arg(a[12]));
+    p.causal = bool_arg(a[11]) ? 1 : 0;
+    size_t nbytes = 0;
+    query("asuka_b200_attn_cache_workspace_bytes", asuka_b200_attn_cache_workspace_bytes(&p, &nbytes));
+    at::Tensor ws;
+    if (nbytes > 0) {
+      ws = empty({static_cast<int64_t>(nbytes)}, at::kByte, q);
+      p.workspace = ws.data_ptr();
+      p.workspace_bytes = nbytes;
+    }
+    call("asuka_b200_attn_cache", [&] { return asuka_b200_attn_cache(&p, on.stream); });
+    if (q0.dim() == 2) out = out.view(q0.sizes());
+    return want_lse ? tuple({wrap(out), wrap(lse)}) : wrap(out);
+  } catch (const BadArg&) {
+    return nullptr;
+  }
+  END_HANDLE_TH_ERRORS
+}
+
 // (q, k, lse, mode, causal, softmax_scale, exp_rand, tau, seed, corm_mask, unit_offset) -> (score, score_sq)
 PyObject* col_scores(PyObject*, PyObject* const* a, Py_ssize_t n) {
   HANDLE_TH_ERRORS
@@ -541,7 +656,8 @@ PyObject* select_topk(PyObject*, PyObject* const* a, Py_ssize_t n) {
 #define ENTRY(f) {#f, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(f)), METH_FASTCALL, nullptr}
 PyMethodDef g_methods[] = {ENTRY(attn_fwd),    ENTRY(run_case),  ENTRY(linear_fwd), ENTRY(linattn32_fwd),
                            ENTRY(pool_scores), ENTRY(gather_kv), ENTRY(col_scores), ENTRY(select_topk),
-                           ENTRY(linear),      ENTRY(linattn_block),
+                           ENTRY(linear),      ENTRY(linattn_block), ENTRY(quant_kv), ENTRY(dequant_kv),
+                           ENTRY(attn_cache),
                            {nullptr, nullptr, 0, nullptr}};
 PyModuleDef g_module = {PyModuleDef_HEAD_INIT, "_bind", nullptr, -1, g_methods, nullptr, nullptr, nullptr, nullptr};
 

@@ -655,6 +655,212 @@ int case_impl(const asuka_case_params* p, CaseKind kind, void* ws, size_t ws_byt
   return r;
 }
 
+// ---- a generation's cache -----------------------------------------------------------------------
+bool is_8bit(int dt) { return dt == ASUKA_I8 || dt == ASUKA_E4M3; }
+
+// The stride of a dimension of one element says nothing and may be anything: the size of a row, which suits every check.
+void plain_strides(asuka_tensor* t, int64_t stride) {
+  for (int i = 0; i < t->ndim - 1 && i < 4; ++i)
+    if (t->shape[i] == 1) t->stride[i] = stride;
+}
+
+// [N, S, H, 128] rows of 16 or 8 bits
+int check_rows(asuka_tensor* t, int dtype) {
+  if (t->ptr == nullptr) return ASUKA_ERR_NULL_POINTER;
+  if (t->dtype != dtype) return ASUKA_ERR_BAD_DTYPE;
+  if (t->ndim != 4) return ASUKA_ERR_BAD_SHAPE;
+  plain_strides(t, kHeadDim);
+  const int r = check_bshd(*t, dtype);
+  if (r != ASUKA_OK) return r;
+  for (int i = 0; i < 3; ++i) {
+    if (is_8bit(dtype) && (t->stride[i] % 16) != 0) return ASUKA_ERR_BAD_STRIDE;
+    if (t->stride[i] > (int64_t{1} << 36)) return ASUKA_ERR_TOO_LARGE;  // (a tensor map's strides have 40 bits, in bytes)
+  }
+  return ASUKA_OK;
+}
+
+int check_scale(asuka_tensor* t, const asuka_tensor& rows) {
+  if (t->ptr == nullptr) return ASUKA_ERR_NULL_POINTER;
+  if (t->dtype != ASUKA_F32) return ASUKA_ERR_BAD_DTYPE;
+  if (t->ndim != 3 || t->shape[0] != rows.shape[0] || t->shape[1] != rows.shape[2] || t->shape[2] != rows.shape[1])
+    return ASUKA_ERR_BAD_SHAPE;
+  plain_strides(t, 4);
+  if (t->shape[2] != 1 && t->stride[2] != 1) return ASUKA_ERR_BAD_STRIDE;
+  for (int i = 0; i < 2; ++i) {
+    if (t->stride[i] <= 0 || (t->stride[i] % 4) != 0) return ASUKA_ERR_BAD_STRIDE;
+    if (t->stride[i] > (int64_t{1} << 36)) return ASUKA_ERR_TOO_LARGE;
+  }
+  if ((reinterpret_cast<uintptr_t>(t->ptr) & 15u) != 0) return ASUKA_ERR_MISALIGNED;
+  return ASUKA_OK;
+}
+
+// optional [n] i32
+int check_counts(const asuka_tensor& t, int64_t n, const int32_t** out) {
+  *out = nullptr;
+  if (t.ptr == nullptr) return ASUKA_OK;
+  if (t.dtype != ASUKA_I32) return ASUKA_ERR_BAD_DTYPE;
+  if (t.ndim != 1 || t.shape[0] != n) return ASUKA_ERR_BAD_SHAPE;
+  if (n != 1 && t.stride[0] != 1) return ASUKA_ERR_BAD_STRIDE;
+  if ((reinterpret_cast<uintptr_t>(t.ptr) & 3u) != 0) return ASUKA_ERR_MISALIGNED;
+  *out = static_cast<const int32_t*>(t.ptr);
+  return ASUKA_OK;
+}
+
+// optional [B, H, n] i32
+int check_idx(const asuka_tensor& t, int64_t B, int64_t H, const int32_t** out, int64_t* n) {
+  *out = nullptr;
+  if (t.ptr == nullptr) return ASUKA_OK;
+  if (t.ndim != 3 || t.shape[2] <= 0) return ASUKA_ERR_BAD_SHAPE;
+  if (t.shape[2] > (1 << 24)) return ASUKA_ERR_TOO_LARGE;
+  const int64_t shape[3] = {B, H, t.shape[2]};
+  const int r = check_dense(t, ASUKA_I32, 3, shape);
+  if (r != ASUKA_OK) return r;
+  *out = static_cast<const int32_t*>(t.ptr);
+  *n = t.shape[2];
+  return ASUKA_OK;
+}
+
+// `dtype16`: what a 16-bit cache has to hold (-1: 8 bits only)
+int prep_cache(const asuka_kv_cache& c, int dtype16, CacheRows* o) {
+  std::memset(o, 0, sizeof(*o));
+  asuka_tensor k = c.k, v = c.v, ks = c.k_scale, vs = c.v_scale;
+  if (k.ptr == nullptr) return ASUKA_ERR_NULL_POINTER;
+  if (!is_8bit(k.dtype) && k.dtype != dtype16) return ASUKA_ERR_BAD_DTYPE;
+  int r;
+  if ((r = check_rows(&k, k.dtype)) != ASUKA_OK) return r;
+  if ((r = check_rows(&v, k.dtype)) != ASUKA_OK) return r;
+  for (int i = 0; i < 4; ++i)
+    if (v.shape[i] != k.shape[i]) return ASUKA_ERR_BAD_SHAPE;
+  if (is_8bit(k.dtype)) {
+    if ((r = check_scale(&ks, k)) != ASUKA_OK) return r;
+    if ((r = check_scale(&vs, k)) != ASUKA_OK) return r;
+    o->k_scale = static_cast<float*>(ks.ptr);
+    o->v_scale = static_cast<float*>(vs.ptr);
+    o->ks_sb = ks.stride[0]; o->ks_sh = ks.stride[1];
+    o->vs_sb = vs.stride[0]; o->vs_sh = vs.stride[1];
+  } else if (ks.ptr != nullptr || vs.ptr != nullptr) {
+    return ASUKA_ERR_BAD_ARGUMENT;
+  }
+  o->k = k.ptr;
+  o->v = v.ptr;
+  o->N = static_cast<int>(k.shape[0]);
+  o->S = static_cast<int>(k.shape[1]);
+  o->format = k.dtype == ASUKA_I8 ? CACHE_I8 : k.dtype == ASUKA_E4M3 ? CACHE_E4M3 : CACHE_16;
+  o->k_sb = k.stride[0]; o->k_ss = k.stride[1]; o->k_sh = k.stride[2];
+  o->v_sb = v.stride[0]; o->v_ss = v.stride[1]; o->v_sh = v.stride[2];
+  return ASUKA_OK;
+}
+
+int prep_quant_kv(const asuka_quant_kv_params* p, QuantKvArgs* a) {
+  if (p == nullptr) return ASUKA_ERR_NULL_POINTER;
+  std::memset(a, 0, sizeof(*a));
+  asuka_tensor k = p->k, v = p->v;
+  if (!is_16bit(k.dtype)) return k.ptr == nullptr ? ASUKA_ERR_NULL_POINTER : ASUKA_ERR_BAD_DTYPE;
+  int r;
+  if ((r = check_rows(&k, k.dtype)) != ASUKA_OK) return r;
+  if ((r = check_rows(&v, k.dtype)) != ASUKA_OK) return r;
+  if ((r = prep_cache(p->cache, -1, &a->cache)) != ASUKA_OK) return r;
+  const int64_t B = k.shape[0], T = k.shape[1], H = k.shape[2];
+  for (int i = 0; i < 4; ++i)
+    if (v.shape[i] != k.shape[i]) return ASUKA_ERR_BAD_SHAPE;
+  if (p->cache.k.shape[0] != B || p->cache.k.shape[2] != H) return ASUKA_ERR_BAD_SHAPE;
+  int64_t n = T;
+  if ((r = check_idx(p->idx, B, H, &a->idx, &n)) != ASUKA_OK) return r;
+  if ((r = check_counts(p->start, B, &a->start)) != ASUKA_OK) return r;
+  if ((r = check_counts(p->count, B, &a->count)) != ASUKA_OK) return r;
+  a->k = static_cast<const uint16_t*>(k.ptr);
+  a->v = static_cast<const uint16_t*>(v.ptr);
+  a->B = static_cast<int>(B); a->H = static_cast<int>(H); a->T = static_cast<int>(T); a->n = static_cast<int>(n);
+  a->k_sb = k.stride[0]; a->k_ss = k.stride[1]; a->k_sh = k.stride[2];
+  a->v_sb = v.stride[0]; a->v_ss = v.stride[1]; a->v_sh = v.stride[2];
+  a->bf16 = k.dtype == ASUKA_BF16;
+  return ASUKA_OK;
+}
+
+int prep_dequant_kv(const asuka_dequant_kv_params* p, DequantKvArgs* a) {
+  if (p == nullptr) return ASUKA_ERR_NULL_POINTER;
+  std::memset(a, 0, sizeof(*a));
+  int r;
+  if ((r = prep_cache(p->cache, -1, &a->cache)) != ASUKA_OK) return r;
+  asuka_tensor k = p->k_out, v = p->v_out;
+  if (!is_16bit(k.dtype)) return k.ptr == nullptr ? ASUKA_ERR_NULL_POINTER : ASUKA_ERR_BAD_DTYPE;
+  if ((r = check_rows(&k, k.dtype)) != ASUKA_OK) return r;
+  if ((r = check_rows(&v, k.dtype)) != ASUKA_OK) return r;
+  const int64_t N = p->cache.k.shape[0], S = p->cache.k.shape[1], H = p->cache.k.shape[2];
+  int64_t n = k.shape[1];
+  if ((r = check_idx(p->idx, N, H, &a->idx, &n)) != ASUKA_OK) return r;
+  if (a->idx == nullptr && n > S) return ASUKA_ERR_BAD_SHAPE;
+  if (k.shape[0] != N || k.shape[1] != n || k.shape[2] != H) return ASUKA_ERR_BAD_SHAPE;
+  for (int i = 0; i < 4; ++i)
+    if (v.shape[i] != k.shape[i]) return ASUKA_ERR_BAD_SHAPE;
+  if ((r = check_counts(p->len, N, &a->cache.len)) != ASUKA_OK) return r;
+  a->k_out = static_cast<uint16_t*>(k.ptr);
+  a->v_out = static_cast<uint16_t*>(v.ptr);
+  a->H = static_cast<int>(H); a->n = static_cast<int>(n);
+  a->k_sb = k.stride[0]; a->k_ss = k.stride[1]; a->k_sh = k.stride[2];
+  a->v_sb = v.stride[0]; a->v_ss = v.stride[1]; a->v_sh = v.stride[2];
+  a->bf16 = k.dtype == ASUKA_BF16;
+  return ASUKA_OK;
+}
+
+int prep_attn_cache(const asuka_attn_cache_params* p, CacheAttnArgs* a) {
+  if (p == nullptr) return ASUKA_ERR_NULL_POINTER;
+  std::memset(a, 0, sizeof(*a));
+  asuka_tensor q = p->q;
+  if (!is_16bit(q.dtype)) return q.ptr == nullptr ? ASUKA_ERR_NULL_POINTER : ASUKA_ERR_BAD_DTYPE;
+  int r;
+  if ((r = check_rows(&q, q.dtype)) != ASUKA_OK) return r;
+  if ((r = prep_cache(p->cache, q.dtype, &a->own)) != ASUKA_OK) return r;
+  const int64_t B = q.shape[0], Sq = q.shape[1], H = q.shape[2], Hkv = p->cache.k.shape[2];
+  if (p->cache.k.shape[0] != B || Hkv > H || H % Hkv != 0) return ASUKA_ERR_BAD_SHAPE;
+  // (query rows and work items are counted in 32 bits; a tile's rows hold all heads of a group)
+  if (H / Hkv > 128 || B * H > (1 << 24) || B * H * Sq > 0x3fffffff) return ASUKA_ERR_TOO_LARGE;
+  if ((r = check_counts(p->len, B, &a->own.len)) != ASUKA_OK) return r;
+  if (p->prefix.k.ptr != nullptr) {
+    if ((r = prep_cache(p->prefix, q.dtype, &a->prefix)) != ASUKA_OK) return r;
+    if (p->prefix.k.shape[2] != Hkv || p->prefix.k.shape[0] > B || B % p->prefix.k.shape[0] != 0) return ASUKA_ERR_BAD_SHAPE;
+    if ((r = check_counts(p->prefix_len, p->prefix.k.shape[0], &a->prefix.len)) != ASUKA_OK) return r;
+  } else if (p->prefix_len.ptr != nullptr) {
+    return ASUKA_ERR_BAD_ARGUMENT;
+  }
+  if (std::isnan(p->softmax_scale) || std::isinf(p->softmax_scale)) return ASUKA_ERR_BAD_ARGUMENT;
+  a->q = static_cast<const uint16_t*>(q.ptr);
+  a->q_sb = q.stride[0]; a->q_ss = q.stride[1]; a->q_sh = q.stride[2];
+  a->B = static_cast<int>(B); a->Sq = static_cast<int>(Sq); a->H = static_cast<int>(H);
+  a->group = static_cast<int>(H / Hkv);
+  a->softmax_scale = p->softmax_scale > 0.f ? p->softmax_scale : 1.0f / std::sqrt(static_cast<float>(kHeadDim));
+  a->causal = p->causal ? 1 : 0;
+  a->bf16 = q.dtype == ASUKA_BF16;
+  return ASUKA_OK;
+}
+
+int attn_cache_impl(const asuka_attn_cache_params* p, cudaStream_t stream) {
+  CacheAttnArgs a;
+  int r = prep_attn_cache(p, &a);
+  if (r != ASUKA_OK) return r;
+  asuka_tensor out = p->out;
+  if ((r = check_rows(&out, p->q.dtype)) != ASUKA_OK) return r;
+  for (int i = 0; i < 4; ++i)
+    if (out.shape[i] != p->q.shape[i]) return ASUKA_ERR_BAD_SHAPE;
+  a.out = static_cast<uint16_t*>(out.ptr);
+  a.o_sb = out.stride[0]; a.o_ss = out.stride[1]; a.o_sh = out.stride[2];
+  if (p->lse.ptr != nullptr) {
+    const int64_t shape[3] = {a.B, a.H, a.Sq};
+    if ((r = check_dense(p->lse, ASUKA_F32, 3, shape)) != ASUKA_OK) return r;
+    a.lse2 = static_cast<float*>(p->lse.ptr);
+  }
+  if ((r = check_arch()) != ASUKA_OK) return r;
+  const int sms = sm_count();
+  if (sms <= 0) return ASUKA_ERR_CUDA;
+  const size_t need = attn_cache_ws_bytes(a, sms);
+  if (need > 0) {
+    if (p->workspace == nullptr) return ASUKA_ERR_NULL_POINTER;
+    if ((reinterpret_cast<uintptr_t>(p->workspace) & 255u) != 0) return ASUKA_ERR_MISALIGNED;
+    if (p->workspace_bytes < need) return ASUKA_ERR_WORKSPACE_TOO_SMALL;
+  }
+  return map_cuda(launch_attn_cache(a, p->workspace, sms, stream));
+}
+
 // ---- scratch for asuka_b200_h2o_static -------------------------------------------------------
 // The array lives in the library's device image: one copy per GPU that loads the library.
 // In HOST code the name `g_h2o_static_scratch` is only a handle for the runtime, not a device
@@ -854,6 +1060,35 @@ int asuka_b200_gather_kv(const asuka_gather_params* p, asuka_stream stream) {
   a.in_sb = p->k.stride[0]; a.in_ss = p->k.stride[1]; a.in_sh = p->k.stride[2];
   a.out_sb = p->k_out.stride[0]; a.out_ss = p->k_out.stride[1]; a.out_sh = p->k_out.stride[2];
   return map_cuda(launch_gather_kv(a, static_cast<cudaStream_t>(stream)));
+}
+
+int asuka_b200_quant_kv(const asuka_quant_kv_params* p, asuka_stream stream) {
+  QuantKvArgs a;
+  int r;
+  if ((r = prep_quant_kv(p, &a)) != ASUKA_OK || (r = check_arch()) != ASUKA_OK) return r;
+  return map_cuda(launch_quant_kv(a, static_cast<cudaStream_t>(stream)));
+}
+
+int asuka_b200_dequant_kv(const asuka_dequant_kv_params* p, asuka_stream stream) {
+  DequantKvArgs a;
+  int r;
+  if ((r = prep_dequant_kv(p, &a)) != ASUKA_OK || (r = check_arch()) != ASUKA_OK) return r;
+  return map_cuda(launch_dequant_kv(a, static_cast<cudaStream_t>(stream)));
+}
+
+int asuka_b200_attn_cache(const asuka_attn_cache_params* p, asuka_stream stream) {
+  return attn_cache_impl(p, static_cast<cudaStream_t>(stream));
+}
+
+int asuka_b200_attn_cache_workspace_bytes(const asuka_attn_cache_params* p, size_t* bytes) {
+  if (p == nullptr || bytes == nullptr) return ASUKA_ERR_NULL_POINTER;
+  CacheAttnArgs a;
+  const int r = prep_attn_cache(p, &a);
+  if (r != ASUKA_OK) return r;
+  const int sms = sm_count();
+  if (sms <= 0) return ASUKA_ERR_CUDA;
+  *bytes = attn_cache_ws_bytes(a, sms);
+  return ASUKA_OK;
 }
 
 int asuka_b200_sima_workspace_bytes(const asuka_sima_params* p, size_t* bytes) {

@@ -152,6 +152,56 @@ struct GatherArgs {
 };
 cudaError_t launch_gather_kv(const GatherArgs& a, cudaStream_t stream);
 
+// One KV cache of `N` sequences of `S` rows: 16-bit values of q's type, or 8-bit codes with a scale for each
+// row.  Strides in elements.
+enum CacheFormat { CACHE_16 = 0, CACHE_I8 = 1, CACHE_E4M3 = 2 };
+struct CacheRows {
+  void* k;
+  void* v;
+  float* k_scale;  // [N, Hkv, S]
+  float* v_scale;
+  const int32_t* len;  // [N] or null
+  int N, S, format;
+  int64_t k_sb, k_ss, k_sh, v_sb, v_ss, v_sh, ks_sb, ks_sh, vs_sb, vs_sh;
+};
+struct QuantKvArgs {
+  const uint16_t* k;
+  const uint16_t* v;
+  const int32_t* idx;  // [B, H, n] or null
+  const int32_t* start;
+  const int32_t* count;
+  CacheRows cache;
+  int B, H, T, n;
+  int64_t k_sb, k_ss, k_sh, v_sb, v_ss, v_sh;
+  bool bf16;
+};
+cudaError_t launch_quant_kv(const QuantKvArgs& a, cudaStream_t stream);
+struct DequantKvArgs {
+  CacheRows cache;
+  const int32_t* idx;
+  uint16_t* k_out;
+  uint16_t* v_out;
+  int H, n;
+  int64_t k_sb, k_ss, k_sh, v_sb, v_ss, v_sh;
+  bool bf16;
+};
+cudaError_t launch_dequant_kv(const DequantKvArgs& a, cudaStream_t stream);
+
+// Attention over a cache and, with prefix.N > 0, over prefixes that B / prefix.N consecutive sequences share.
+struct CacheAttnArgs {
+  const uint16_t* q;
+  uint16_t* out;
+  float* lse2;  // or null
+  int64_t q_sb, q_ss, q_sh, o_sb, o_ss, o_sh;
+  int B, Sq, H, group;
+  CacheRows own, prefix;
+  float softmax_scale;
+  int causal;
+  bool bf16;
+};
+size_t attn_cache_ws_bytes(const CacheAttnArgs& a, int num_sms);
+cudaError_t launch_attn_cache(const CacheAttnArgs& a, void* ws, int num_sms, cudaStream_t stream);
+
 // linear attention at head_dim 32, f32: q, k, v, out [B, N, H, 32], strides in elements (unit stride
 // along the features, the others multiples of 4)
 struct LinAttn32Args {

@@ -14,7 +14,8 @@ from . import _lib
 from ._lib import AsukaError  # noqa: F401  (re-exported)
 
 _DTYPES = {torch.float16: _lib.F16, torch.bfloat16: _lib.BF16, torch.float32: _lib.F32,
-           torch.int32: _lib.I32, torch.uint8: _lib.U8, torch.bool: _lib.U8}
+           torch.int32: _lib.I32, torch.uint8: _lib.U8, torch.bool: _lib.U8, torch.int8: _lib.I8,
+           torch.float8_e4m3fn: _lib.E4M3}
 
 
 _native = None
@@ -138,6 +139,39 @@ def pool_scores(score, kernel_size):
 def gather_kv(k, v, idx):
   """Compact the KV cache to the kept keys: (k[b, idx[b,h,n], h, :], v alike) as [B, n, H, 128]."""
   return _bind().gather_kv(k, v, idx)
+
+
+def quant_kv(k, v, cache, start=None, count=None, idx=None):
+  """Write k and v [B, T, Hkv, 128] (f16 or bf16) into an 8-bit ``KVCache`` of the same B sequences: row i of
+  sequence b becomes the cache's row start[b] + i (``start`` [B] int32, default 0).  With ``idx`` [B, Hkv, n]
+  int32, as a selection returns it, the n rows are k[b, idx[b, h, i], h] instead (indices are clamped as in
+  ``gather_kv``).  ``count`` [B] int32: only the first count[b] rows are real, the rest is padding and is not
+  written, nor is a row that would land outside the cache; all other rows of the cache stay as they are."""
+  _bind().quant_kv(k, v, cache.k, cache.v, cache.k_scale, cache.v_scale, start, count, idx)
+
+
+def dequant_kv(cache, dtype=torch.bfloat16, idx=None, kv_len=None, length=None):
+  """The rows of an 8-bit ``KVCache`` as 16-bit values, (k, v) [B, n, Hkv, 128]: the first ``length`` rows
+  (default: all), or the rows ``idx`` [B, Hkv, n] int32.  Rows from kv_len[b] on read as 0."""
+  return _bind().dequant_kv(cache.k, cache.v, cache.k_scale, cache.v_scale, dtype, idx, kv_len,
+                            -1 if length is None else length)
+
+
+def attn_cache(q, cache, kv_len=None, causal=True, softmax_scale=0.0, return_lse=False, out=None):
+  """Attention of new tokens q [B, Sq, H, 128] over a ``KVCache`` in which sequence b has kv_len[b] rows
+  (int32 [B]; default: all), the new tokens' own among them: row i sees j <= i + kv_len[b] - Sq (causal) or
+  all of kv_len[b].  A row that sees nothing gives 0.  With ``return_lse`` also the base-2 log-sum-exp [B, H, Sq]."""
+  return _bind().attn_cache(q, cache.k, cache.v, cache.k_scale, cache.v_scale, kv_len, None, None, None, None, None,
+                            causal, softmax_scale, return_lse, out)
+
+
+def attn_prefix(q, prefix, cache, kv_len=None, prefix_len=None, causal=True, softmax_scale=0.0, return_lse=False,
+                out=None):
+  """``attn_cache`` for sequences that share a prefix: ``prefix`` is a ``KVCache`` of G sequences, each seen in
+  full (prefix_len[g] rows; int32 [G], default: all) by the B / G consecutive sequences behind it, ahead of
+  their own rows in ``cache``; it is read once for all of them.  One softmax goes over both."""
+  return _bind().attn_cache(q, cache.k, cache.v, cache.k_scale, cache.v_scale, kv_len, prefix.k, prefix.v,
+                            prefix.k_scale, prefix.v_scale, prefix_len, causal, softmax_scale, return_lse, out)
 
 
 def sima_fwd(q, k, v, out_dtype=None):

@@ -50,7 +50,7 @@ typedef enum {
   ASUKA_ERR_TOO_LARGE = -11
 } asuka_status;
 
-typedef enum { ASUKA_F16 = 0, ASUKA_BF16 = 1, ASUKA_F32 = 2, ASUKA_I32 = 3, ASUKA_U8 = 4 } asuka_dtype;
+typedef enum { ASUKA_F16 = 0, ASUKA_BF16 = 1, ASUKA_F32 = 2, ASUKA_I32 = 3, ASUKA_U8 = 4, ASUKA_I8 = 5, ASUKA_E4M3 = 6 } asuka_dtype;
 
 typedef struct {
   void* ptr;
@@ -175,6 +175,64 @@ typedef struct {
   asuka_tensor k, v, idx, k_out, v_out;
 } asuka_gather_params;
 int asuka_b200_gather_kv(const asuka_gather_params* p, asuka_stream stream);
+
+/* ---- a generation's KV cache: the rows of N sequences, `S` to each, in 16 bits or in 8 -----------
+ * The reference has no counterpart (it stops at prefill and scores).  In 8 bits a row -- a token's
+ * key or value of one head, 128 values -- is its codes times one scale:
+ *     scale = max(amax, M * 2^-100) / M,   code = round_to_even(x * M / max(amax, M * 2^-100))
+ * with amax the row's largest magnitude and M = 127 (ASUKA_I8) or 448 (ASUKA_E4M3, rounded to that
+ * type).  A row with an infinity or a NaN gets the scale NaN and codes 0, and reads back as NaN. ---- */
+typedef struct {
+  asuka_tensor k;       /* [N, S, Hkv, 128] f16 | bf16 | i8 | e4m3; base and strides multiples of 16 bytes */
+  asuka_tensor v;       /* the same shape and type, strides of its own */
+  asuka_tensor k_scale; /* 8-bit caches: [N, Hkv, S] f32, unit stride along S, the other strides multiples */
+  asuka_tensor v_scale; /* of 4 elements, 16-byte aligned; 16-bit caches: ptr NULL */
+} asuka_kv_cache;
+
+/* Writes rows into an 8-bit cache: row i of sequence b and head h goes to row start[b] + i, from row i
+ * of k and v or, with idx, from row idx[b, h, i] (clamped to [0, T)): the compaction of a selection.
+ * Rows from count[b] on (padding) and rows that would land outside [0, S) are not written. */
+typedef struct {
+  asuka_tensor k, v;    /* [B, T, Hkv, 128] f16 | bf16, same type, strides as for asuka_b200_attn_fwd */
+  asuka_tensor idx;     /* optional: [B, Hkv, n] i32, contiguous (n rows are written instead of T) */
+  asuka_tensor start;   /* optional: [B] i32, contiguous; absent: 0 */
+  asuka_tensor count;   /* optional: [B] i32, contiguous; absent: all rows */
+  asuka_kv_cache cache; /* N = B; must not overlap k and v */
+} asuka_quant_kv_params;
+int asuka_b200_quant_kv(const asuka_quant_kv_params* p, asuka_stream stream);
+
+/* Reads rows of an 8-bit cache back as code * scale, rounded once to the output's type: rows 0 .. n - 1,
+ * or rows idx[b, h, i] (clamped to [0, S)).  Rows from len[b] on read as 0. */
+typedef struct {
+  asuka_kv_cache cache;
+  asuka_tensor idx;          /* optional: [N, Hkv, n] i32, contiguous */
+  asuka_tensor len;          /* optional: [N] i32, contiguous */
+  asuka_tensor k_out, v_out; /* [N, n, Hkv, 128] f16 | bf16, same type, n <= S without idx */
+} asuka_dequant_kv_params;
+int asuka_b200_dequant_kv(const asuka_dequant_kv_params* p, asuka_stream stream);
+
+/* Attention of new tokens over such a cache, and over the prefix that sequences share:
+ *   - query row i of sequence b sees row j of its own cache iff j < len[b] and, with causal,
+ *     j <= i + len[b] - Sq (the new tokens' own rows are the cache's last Sq);
+ *   - the prefix (optional) holds G sequences, each shared by B / G consecutive sequences of q, which
+ *     see all of its first prefix_len[g] rows.
+ * One softmax goes over both; a row that sees nothing is 0 with the log-sum-exp -inf.  Lengths are
+ * clamped to [0, S].  The cache and the prefix may be of different types; a 16-bit one has q's. */
+typedef struct {
+  asuka_tensor q;            /* [B, Sq, H, 128] f16 | bf16; H a multiple of the cache's heads, H / Hkv <= 128 */
+  asuka_tensor out;          /* like q */
+  asuka_tensor lse;          /* optional: [B, H, Sq] f32, contiguous: base-2 log-sum-exp of the scaled logits */
+  asuka_kv_cache cache;      /* N = B */
+  asuka_tensor len;          /* optional: [B] i32, contiguous; absent: S */
+  asuka_kv_cache prefix;     /* optional (k.ptr NULL: none): N = G, a divisor of B; the same heads */
+  asuka_tensor prefix_len;   /* optional: [G] i32, contiguous; absent: the prefix's S */
+  float softmax_scale;       /* <= 0 selects 1/sqrt(128) */
+  int32_t causal;
+  void* workspace;           /* asuka_b200_attn_cache_workspace_bytes, 256-byte aligned: partial results */
+  uint64_t workspace_bytes;
+} asuka_attn_cache_params;
+int asuka_b200_attn_cache(const asuka_attn_cache_params* p, asuka_stream stream);
+int asuka_b200_attn_cache_workspace_bytes(const asuka_attn_cache_params* p, size_t* bytes);
 
 /* ---- SimA softmax-free attention: replaces the generated kernels for bench/sima.mlir:13-17
  *      (L1 normalisation as lib/Dialect/Asuka/Transforms/LowerComplexReduce.cpp:44-69). ---- */
