@@ -47,6 +47,21 @@ inline int make_bshd_map(CUtensorMap* map, const void* base, bool is_bf16, int64
   return r == CUDA_SUCCESS ? 0 : (int)r;
 }
 
+// The same tensor of bytes (8-bit codes): boxes of all 128 columns, so that a row is one swizzled row of 128 bytes.
+inline int make_bshd_bytes_map(CUtensorMap* map, const void* base, int64_t B, int64_t S, int64_t H, int64_t stride_b,
+                               int64_t stride_s, int64_t stride_h, uint32_t box_rows) {
+  encode_tiled_fn fn = get_encode_fn();
+  if (!fn) return -1;
+  cuuint64_t dims[4] = {128, (cuuint64_t)H, (cuuint64_t)S, (cuuint64_t)B};
+  cuuint64_t strides[3] = {(cuuint64_t)stride_h, (cuuint64_t)stride_s, (cuuint64_t)stride_b};
+  cuuint32_t box[4] = {128, 1, box_rows, 1};
+  cuuint32_t estr[4] = {1, 1, 1, 1};
+  CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, const_cast<void*>(base), dims, strides, box, estr,
+                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? 0 : (int)r;
+}
+
 // A 4-D f32 tensor (innermost stride 1; `strides` in BYTES for dimensions 1..3, multiples of 16),
 // box[0] = 32 elements (128 bytes), with or without the 128-byte swizzle.  Out-of-range elements read
 // as zero and are dropped on store.  Returns 0 on success.
