@@ -19,134 +19,10 @@
 //   - a key's scale multiplies its logits; a value's scale s multiplies the weights, w s = exp2(x) s, rounded to f16.  The reference of
 //     the exponentials is the largest x + log2(s), so w s <= 1 and the rounding is 2^-11 of it (2^-25 of the largest where it is
 //     subnormal).
-#include <cuda_bf16.h>
-#include <cuda_fp16.h>
-#include <cuda_fp8.h>
-
-#include <type_traits>
-
-#include "kernels.h"
-#include "sm100_ptx.cuh"
-#include "tma_host.h"
+#include "attn_cache.cuh"
 
 namespace asuka {
-using namespace sm100;
-
 namespace {
-
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-__device__ __forceinline__ float lg2(float x) {
-  float y;
-  asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-template <bool kBF16>
-__device__ __forceinline__ float2 unpack2(uint32_t w) {
-  if constexpr (kBF16) return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&w));
-  else return __half22float2(*reinterpret_cast<const __half2*>(&w));
-}
-template <bool kBF16>
-__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
-  if constexpr (kBF16) {
-    const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
-    return *reinterpret_cast<const uint32_t*>(&v);
-  } else {
-    const __half2 v = __floats2half2_rn(lo, hi);
-    return *reinterpret_cast<const uint32_t*>(&v);
-  }
-}
-
-// ---- a segment's rows ----------------------------------------------------------------------------
-struct Segment {
-  int N, S, n;     // sequences, rows of each at most, sequences of q to each
-  int rows;        // query rows of a unit: n * Sq * group
-  int causal;
-  const int32_t* len;
-};
-struct RowShape {
-  int Sq, H, Hkv, group;
-};
-// Row r of a unit: (sequence of q, position, head in the group), heads fastest.
-struct Row {
-  int b, pos, h;
-};
-__device__ __forceinline__ Row decode_row(int r, int seq, int hk, const Segment& s, const RowShape& q) {
-  const int g = r % q.group, x = r / q.group;
-  return {seq * s.n + x / q.Sq, x % q.Sq, hk * q.group + g};
-}
-__device__ __forceinline__ int seen_of(const Segment& s, int seq) {
-  return s.len != nullptr ? min(max(s.len[seq], 0), s.S) : s.S;
-}
-// Partial results of a query row, numbered in the output's own order: `parts` of each, in part order.
-struct Partials {
-  float* o;   // [B * Sq * H][parts][128], unnormalised
-  float* ml;  // [B * Sq * H][parts][2]: reference of the exponentials (-inf: nothing seen) and their sum
-  int parts;
-};
-
-constexpr int kThreads = 128;
-
-// four values of row `off` (elements) from column 4 lane on
-template <bool kBF16>
-__device__ __forceinline__ float4 load4(const void* base, int64_t off, int lane, int format) {
-  if (format == CACHE_16) {
-    const uint2 w = reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(base) + off)[lane];
-    const float2 a = unpack2<kBF16>(w.x), b = unpack2<kBF16>(w.y);
-    return make_float4(a.x, a.y, b.x, b.y);
-  }
-  const uint32_t w = reinterpret_cast<const uint32_t*>(static_cast<const uint8_t*>(base) + off)[lane];
-  if (format == CACHE_I8)
-    return make_float4(static_cast<int8_t>(w), static_cast<int8_t>(w >> 8), static_cast<int8_t>(w >> 16), static_cast<int8_t>(w >> 24));
-  const __half2 lo(__nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(w & 0xffffu), __NV_E4M3));
-  const __half2 hi(__nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(w >> 16), __NV_E4M3));
-  const float2 a = __half22float2(lo), b = __half22float2(hi);
-  return make_float4(a.x, a.y, b.x, b.y);
-}
-
-template <bool kBF16>
-__global__ void __launch_bounds__(kThreads) attn_cache_kernel(const CacheAttnArgs a) {
-  const int lane = threadIdx.x & 31;
-  const int64_t row = static_cast<int64_t>(blockIdx.x) * (kThreads / 32) + (threadIdx.x >> 5);
-  griddep_wait();
-  griddep_launch_dependents();
-  if (row >= static_cast<int64_t>(a.B) * a.Sq * a.H) return;
-  const int h = static_cast<int>(row % a.H), i = static_cast<int>(row / a.H % a.Sq), b = static_cast<int>(row / a.H / a.Sq);
-  const int hk = h / a.group;
-  const float4 q = load4<kBF16>(a.q, b * a.q_sb + i * a.q_ss + h * a.q_sh, lane, CACHE_16);
-  const float mul = a.softmax_scale * 1.4426950408889634f;
-  float m = -INFINITY, l = 0.f;
-  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int which = 0; which < 2; ++which) {
-    const CacheRows& c = which == 0 ? a.prefix : a.own;
-    if (c.N == 0) continue;
-    const int n = b / (a.B / c.N);
-    int seen = c.len != nullptr ? min(max(c.len[n], 0), c.S) : c.S;
-    if (which == 1 && a.causal) seen = min(seen, seen - a.Sq + 1 + i);
-    for (int64_t j = 0; j < seen; ++j) {
-      const float4 k = load4<kBF16>(c.k, n * c.k_sb + j * c.k_ss + hk * c.k_sh, lane, c.format);
-      float s = q.x * k.x + q.y * k.y + q.z * k.z + q.w * k.w;
-#pragma unroll
-      for (int d = 16; d > 0; d >>= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
-      s *= mul;
-      if (c.format != CACHE_16) s *= c.k_scale[n * c.ks_sb + hk * c.ks_sh + j];
-      const float top = fmaxf(m, s), ref = top > -INFINITY ? top : 0.f;
-      const float w = ex2(m - ref), p = ex2(s - ref);
-      m = top;
-      l = l * w + p;
-      const float pv = c.format != CACHE_16 ? p * c.v_scale[n * c.vs_sb + hk * c.vs_sh + j] : p;
-      const float4 v = load4<kBF16>(c.v, n * c.v_sb + j * c.v_ss + hk * c.v_sh, lane, c.format);
-      o = make_float4(fmaf(pv, v.x, o.x * w), fmaf(pv, v.y, o.y * w), fmaf(pv, v.z, o.z * w), fmaf(pv, v.w, o.w * w));
-    }
-  }
-  const float inv = l == 0.f ? 0.f : 1.f / l;
-  reinterpret_cast<uint2*>(a.out + b * a.o_sb + i * a.o_ss + h * a.o_sh)[lane] =
-      make_uint2(pack2<kBF16>(o.x * inv, o.y * inv), pack2<kBF16>(o.z * inv, o.w * inv));
-  if (a.lse2 != nullptr && lane == 0) a.lse2[(static_cast<int64_t>(b) * a.H + h) * a.Sq + i] = m + log2f(l);
-}
 
 // ---- up to 16 rows to a unit -----------------------------------------------------------------------
 constexpr int kRows = 16;
@@ -228,22 +104,6 @@ __device__ __forceinline__ float ld_cluster(uint32_t smem_addr, uint32_t rank) {
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(smem_addr), "r"(rank));
   asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(remote) : "memory");
   return v;
-}
-
-// Codes of four consecutive bytes as f16 pairs: (0, 1) and (2, 3).
-template <int kFmt>
-__device__ __forceinline__ void codes_to_f16(uint32_t w, uint32_t& lo, uint32_t& hi) {
-  if constexpr (kFmt == CACHE_E4M3) {
-    asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\t"
-        "cvt.rn.f16x2.e4m3x2 %0, a;\n\tcvt.rn.f16x2.e4m3x2 %1, b;\n\t}" : "=r"(lo), "=r"(hi) : "r"(w));
-  } else {
-    const uint32_t u = w ^ 0x80808080u;
-    const __half2 off = __floats2half2_rn(1152.f, 1152.f);
-    uint32_t a = __byte_perm(u, 0x64646464u, 0x4140), b = __byte_perm(u, 0x64646464u, 0x4342);
-    const __half2 x = __hsub2(*reinterpret_cast<__half2*>(&a), off), y = __hsub2(*reinterpret_cast<__half2*>(&b), off);
-    lo = *reinterpret_cast<const uint32_t*>(&x);
-    hi = *reinterpret_cast<const uint32_t*>(&y);
-  }
 }
 
 // Grid: units x parts, the parts of a unit a cluster.  kLast: this segment's results, with what the one before left, are the output.
@@ -631,6 +491,7 @@ attn_stream_kernel(const __grid_constant__ StreamMaps maps, const StreamParams p
       const Row row = decode_row(r, seq, hk, p.s, p.q);
       const int64_t number = (static_cast<int64_t>(row.b) * p.q.Sq + row.pos) * p.q.H + row.h;
       if constexpr (!kLast) {
+        if (!(mm > -INFINITY) && ll != 0.f) mm = 0.f;  // (nothing but NaN: the sum)
         p.mine.o[number * 128 + tid] = acc;
         if (tid == 0) *reinterpret_cast<float2*>(p.mine.ml + number * 2) = make_float2(mm, ll);
       } else {
@@ -654,32 +515,6 @@ attn_stream_kernel(const __grid_constant__ StreamMaps maps, const StreamParams p
     }
   }
   cluster_sync();  // no CTA leaves while another still reads its shared memory
-}
-
-// ---- host side -------------------------------------------------------------------------------------
-Segment segment_of(const CacheRows& c, const CacheAttnArgs& a, bool causal) {
-  Segment s;
-  s.N = c.N;
-  s.S = c.S;
-  s.n = a.B / c.N;
-  s.rows = s.n * a.Sq * a.group;
-  s.causal = causal ? 1 : 0;
-  s.len = c.len;
-  return s;
-}
-
-int make_rows_map(CUtensorMap* m, const CacheRows& c, bool values, int H, bool bf16, uint32_t box_rows) {
-  const void* base = values ? c.v : c.k;
-  const int64_t sb = values ? c.v_sb : c.k_sb, ss = values ? c.v_ss : c.k_ss, sh = values ? c.v_sh : c.k_sh;
-  return c.format == CACHE_16 ? tma_host::make_bshd_map(m, base, bf16, c.N, c.S, H, 128, sb, ss, sh, box_rows)
-                              : tma_host::make_bshd_bytes_map(m, base, c.N, c.S, H, sb, ss, sh, box_rows);
-}
-int make_scale_map(CUtensorMap* m, const CacheRows& c, bool values, int H, uint32_t box) {
-  const uint64_t dims[4] = {static_cast<uint64_t>(c.S), static_cast<uint64_t>(H), static_cast<uint64_t>(c.N), 1};
-  const uint64_t sb = static_cast<uint64_t>(values ? c.vs_sb : c.ks_sb) * 4, sh = static_cast<uint64_t>(values ? c.vs_sh : c.ks_sh) * 4;
-  const uint64_t strides[3] = {sh, sb, sb};
-  const uint32_t boxes[4] = {box, 1, 1, 1};
-  return tma_host::make_f32_map(m, values ? c.v_scale : c.k_scale, dims, strides, boxes, false);
 }
 
 template <int kFmt, bool kLast>
@@ -720,36 +555,49 @@ cudaError_t launch_stream(const CacheRows& c, StreamParams& p, bool bf16, int nu
   }
 }
 
-// Where the prefix's partial results lie in the workspace.
+// Query rows are few enough for the stream's one 16-row tile.
+bool streams(const Segment& s) { return s.rows <= kRows; }
+
+// How the work of a call is cut: the prefix's partial results first in the workspace, then the own rows', where those do not
+// finish it themselves.
+struct Plan {
+  Segment prefix, own;
+  int prefix_parts, own_parts;  // 0: none kept
+};
+Plan plan_of(const CacheAttnArgs& a, int num_sms) {
+  const RowShape q{a.Sq, a.H, a.H / a.group, a.group};
+  Plan x;
+  x.own = segment_of(a.own, a, a.causal != 0);
+  x.own_parts = streams(x.own) ? 0 : attn_rows_parts(x.own, q, num_sms);
+  x.prefix_parts = 0;
+  if (a.prefix.N > 0) {
+    x.prefix = segment_of(a.prefix, a, false);
+    x.prefix_parts = streams(x.prefix) ? 1 : attn_rows_parts(x.prefix, q, num_sms);
+  }
+  return x;
+}
+size_t row_count(const CacheAttnArgs& a) { return static_cast<size_t>(a.B) * a.Sq * a.H; }
+size_t partial_bytes(const CacheAttnArgs& a, int parts) {
+  return (row_count(a) * parts * (128 + 2) * sizeof(float) + 255) / 256 * 256;
+}
 Partials partials_at(void* ws, const CacheAttnArgs& a, int parts) {
   Partials x;
   x.parts = parts;
   x.o = static_cast<float*>(ws);
-  x.ml = x.o + static_cast<size_t>(a.B) * a.Sq * a.H * parts * 128;
+  x.ml = x.o + row_count(a) * parts * 128;
   return x;
-}
-size_t partial_bytes(const CacheAttnArgs& a, int parts) {
-  return static_cast<size_t>(a.B) * a.Sq * a.H * parts * (128 + 2) * sizeof(float);
-}
-bool streams(const CacheAttnArgs& a) {
-  if (a.Sq > kRows || a.Sq * a.group > kRows) return false;
-  return a.prefix.N == 0 || static_cast<int64_t>(a.B / a.prefix.N) * a.Sq * a.group <= kRows;
 }
 
 }  // namespace
 
-size_t attn_cache_ws_bytes(const CacheAttnArgs& a, int) {
-  return streams(a) && a.prefix.N > 0 ? partial_bytes(a, 1) : 0;
+size_t attn_cache_ws_bytes(const CacheAttnArgs& a, int num_sms) {
+  const Plan x = plan_of(a, num_sms);
+  return partial_bytes(a, x.prefix_parts) + partial_bytes(a, x.own_parts);
 }
 
 cudaError_t launch_attn_cache(const CacheAttnArgs& a, void* ws, int num_sms, cudaStream_t stream) {
-  if (!streams(a)) {
-    const int64_t rows = static_cast<int64_t>(a.B) * a.Sq * a.H;
-    const auto kern = a.bf16 ? attn_cache_kernel<true> : attn_cache_kernel<false>;
-    const cudaError_t e = launch_dependent(kern, dim3(static_cast<unsigned>((rows + 3) / 4)), dim3(kThreads), 0, stream, a);
-    count_launch();
-    return e;
-  }
+  const Plan x = plan_of(a, num_sms);
+  const Partials first = partials_at(ws, a, x.prefix_parts);
   StreamParams p;
   p.q = RowShape{a.Sq, a.H, a.H / a.group, a.group};
   p.scale_log2 = a.softmax_scale * 1.4426950408889634f;
@@ -759,15 +607,21 @@ cudaError_t launch_attn_cache(const CacheAttnArgs& a, void* ws, int num_sms, cud
   p.o_sb = a.o_sb; p.o_ss = a.o_ss; p.o_sh = a.o_sh;
   p.lse2 = a.lse2;
   p.status = device_status_words();
-  p.prior = p.mine = Partials{nullptr, nullptr, 0};
-  if (a.prefix.N > 0) {
-    p.mine = p.prior = partials_at(ws, a, 1);
-    p.s = segment_of(a.prefix, a, false);
-    const cudaError_t e = launch_stream<false>(a.prefix, p, a.bf16, num_sms, stream);
+  p.prior = p.mine = first;
+  cudaError_t e = cudaSuccess;
+  if (x.prefix_parts > 0) {
+    p.s = x.prefix;
+    e = streams(x.prefix) ? launch_stream<false>(a.prefix, p, a.bf16, num_sms, stream)
+                          : launch_attn_rows(a.prefix, x.prefix, a, first, num_sms, stream);
     if (e != cudaSuccess) return e;
   }
-  p.s = segment_of(a.own, a, a.causal != 0);
-  return launch_stream<true>(a.own, p, a.bf16, num_sms, stream);
+  if (x.own_parts == 0) {
+    p.s = x.own;
+    return launch_stream<true>(a.own, p, a.bf16, num_sms, stream);
+  }
+  const Partials second = partials_at(static_cast<uint8_t*>(ws) + partial_bytes(a, x.prefix_parts), a, x.own_parts);
+  e = launch_attn_rows(a.own, x.own, a, second, num_sms, stream);
+  return e != cudaSuccess ? e : launch_attn_merge(a, first, second, stream);
 }
 
 }  // namespace asuka

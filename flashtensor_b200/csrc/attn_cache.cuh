@@ -1,0 +1,117 @@
+// What the kernels of attention over caches share: a segment's rows, partial results, codes, tensor maps.
+#pragma once
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "kernels.h"
+#include "sm100_ptx.cuh"
+#include "tma_host.h"
+
+namespace asuka {
+using namespace sm100;
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float lg2(float x) {
+  float y;
+  asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+template <bool kBF16>
+__device__ __forceinline__ float2 unpack2(uint32_t w) {
+  if constexpr (kBF16) return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&w));
+  else return __half22float2(*reinterpret_cast<const __half2*>(&w));
+}
+template <bool kBF16>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+  if constexpr (kBF16) {
+    const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&v);
+  } else {
+    const __half2 v = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&v);
+  }
+}
+
+// ---- a segment's rows ----------------------------------------------------------------------------
+struct Segment {
+  int N, S, n;     // sequences, rows of each at most, sequences of q to each
+  int rows;        // query rows of a unit: n * Sq * group
+  int causal;
+  const int32_t* len;
+};
+struct RowShape {
+  int Sq, H, Hkv, group;
+};
+// Row r of a unit: (sequence of q, position, head in the group), heads fastest.
+struct Row {
+  int b, pos, h;
+};
+__device__ __forceinline__ Row decode_row(int r, int seq, int hk, const Segment& s, const RowShape& q) {
+  const int g = r % q.group, x = r / q.group;
+  return {seq * s.n + x / q.Sq, x % q.Sq, hk * q.group + g};
+}
+__device__ __forceinline__ int seen_of(const Segment& s, int seq) {
+  return s.len != nullptr ? min(max(s.len[seq], 0), s.S) : s.S;
+}
+// Partial results of a query row, numbered in the output's own order: `parts` of each, in part order.
+// (A row that saw nothing but NaN has a NaN sum under the reference 0.)
+struct Partials {
+  float* o;   // [B * Sq * H][parts][128], unnormalised
+  float* ml;  // [B * Sq * H][parts][2]: reference of the exponentials (-inf: nothing seen) and their sum
+  int parts;
+};
+
+// Codes of four consecutive bytes as f16 pairs: (0, 1) and (2, 3).
+template <int kFmt>
+__device__ __forceinline__ void codes_to_f16(uint32_t w, uint32_t& lo, uint32_t& hi) {
+  if constexpr (kFmt == CACHE_E4M3) {
+    asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\t"
+        "cvt.rn.f16x2.e4m3x2 %0, a;\n\tcvt.rn.f16x2.e4m3x2 %1, b;\n\t}" : "=r"(lo), "=r"(hi) : "r"(w));
+  } else {
+    const uint32_t u = w ^ 0x80808080u;
+    const __half2 off = __floats2half2_rn(1152.f, 1152.f);
+    uint32_t a = __byte_perm(u, 0x64646464u, 0x4140), b = __byte_perm(u, 0x64646464u, 0x4342);
+    const __half2 x = __hsub2(*reinterpret_cast<__half2*>(&a), off), y = __hsub2(*reinterpret_cast<__half2*>(&b), off);
+    lo = *reinterpret_cast<const uint32_t*>(&x);
+    hi = *reinterpret_cast<const uint32_t*>(&y);
+  }
+}
+
+// ---- host side -------------------------------------------------------------------------------------
+inline Segment segment_of(const CacheRows& c, const CacheAttnArgs& a, bool causal) {
+  Segment s;
+  s.N = c.N;
+  s.S = c.S;
+  s.n = a.B / c.N;
+  s.rows = s.n * a.Sq * a.group;
+  s.causal = causal ? 1 : 0;
+  s.len = c.len;
+  return s;
+}
+
+inline int make_rows_map(CUtensorMap* m, const CacheRows& c, bool values, int H, bool bf16, uint32_t box_rows) {
+  const void* base = values ? c.v : c.k;
+  const int64_t sb = values ? c.v_sb : c.k_sb, ss = values ? c.v_ss : c.k_ss, sh = values ? c.v_sh : c.k_sh;
+  return c.format == CACHE_16 ? tma_host::make_bshd_map(m, base, bf16, c.N, c.S, H, 128, sb, ss, sh, box_rows)
+                              : tma_host::make_bshd_bytes_map(m, base, c.N, c.S, H, sb, ss, sh, box_rows);
+}
+inline int make_scale_map(CUtensorMap* m, const CacheRows& c, bool values, int H, uint32_t box) {
+  const uint64_t dims[4] = {static_cast<uint64_t>(c.S), static_cast<uint64_t>(H), static_cast<uint64_t>(c.N), 1};
+  const uint64_t sb = static_cast<uint64_t>(values ? c.vs_sb : c.ks_sb) * 4, sh = static_cast<uint64_t>(values ? c.vs_sh : c.ks_sh) * 4;
+  const uint64_t strides[3] = {sh, sb, sb};
+  const uint32_t boxes[4] = {box, 1, 1, 1};
+  return tma_host::make_f32_map(m, values ? c.v_scale : c.k_scale, dims, strides, boxes, false);
+}
+
+// attn_rows.cu: a segment of more than 16 rows to a unit leaves its partial results at `mine` (mine.parts of each row)
+int attn_rows_parts(const Segment& s, const RowShape& q, int num_sms);
+cudaError_t launch_attn_rows(const CacheRows& c, const Segment& s, const CacheAttnArgs& a, const Partials& mine, int num_sms,
+                             cudaStream_t stream);
+// ... and the output is what the partial results of up to two segments add up to
+cudaError_t launch_attn_merge(const CacheAttnArgs& a, const Partials& first, const Partials& second, cudaStream_t stream);
+
+}  // namespace asuka

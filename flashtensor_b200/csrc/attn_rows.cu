@@ -1,0 +1,748 @@
+// Attention of many query rows to a unit over a cache or a shared prefix (attn_cache.cu has the segments, units and partial
+// results, and the kernel for up to 16 rows).
+//
+// The rows of all sequences that share a prefix -- times their new positions, times the heads of a group -- are rows of one
+// matrix product with its keys: tiles of 128 (a tensor map whose box is group x positions x sequences gathers them), so that a
+// key is read and multiplied once for all of them.  A CTA takes one or two tiles and a part of the keys:
+//   warp 0        TMA: Q once, K (8-bit caches: the codes of K and V in turn, and their scales)
+//   warp 2        TMA: V
+//   warp 1        issues S = Q_t K^T (tcgen05.mma, SMEM x SMEM)
+//   warp 3        issues O_t += P_t V (TMEM x SMEM)
+//   warps 4-11    softmax, a thread to a row of S
+//   warps 12-15   (8-bit caches) codes to 16-bit tiles
+// The two softmax slots ping-pong as in attn_fwd.cu, one S in tensor memory serving both: with two tiles each has one of them and a K/V
+// tile serves both; with one tile a slot has the even key tiles and the other the odd ones, merged at the end.  What is left of a
+// part goes to the workspace unnormalised.
+//
+// 8-bit codes are brought to q's type times their row's scale, rounded once (2^-9 of a value in bf16, 2^-12 in f16, as the
+// cache read back would be): a thread takes one row's 128 codes from the swizzled stage and writes them in the two swizzled halves the
+// tensor pipe reads, neither with a bank conflict.
+#include "attn_cache.cuh"
+
+namespace asuka {
+
+namespace {
+
+constexpr int kTile = 128;
+constexpr uint32_t kTileBytes = 128 * 128 * 2;  // [128 x 128] 16-bit: two swizzled halves
+constexpr uint32_t kHalfBytes = kTileBytes / 2;
+constexpr uint32_t kRawBytes = 128 * 128;       // [128 x 128] codes
+constexpr float kRescaleLimit = 6.0f;           // log2 of the largest exponential tolerated under a stale reference
+
+// kPair: two query tiles; else one.  Shared memory: Q, the rings of 16-bit K and V tiles, of codes, of their scales.
+template <int kFmt, bool kPair> struct Cfg {
+  static constexpr bool k8 = kFmt != CACHE_16;
+  static constexpr int kQ = kPair ? 2 : 1;
+  static constexpr int kK = k8 ? 2 : 3;
+  static constexpr int kV = k8 ? 2 : (kPair ? 2 : 3);
+  static constexpr int kRaw = k8 ? (kPair ? 2 : 3) : 0;
+  static constexpr uint32_t kSmem = (kQ + kK + kV) * kTileBytes + kRaw * (kRawBytes + 512) + 1024;
+  static constexpr int kThreads = k8 ? 512 : 384;
+  // setmaxnreg: what the roles ask for is what the block gets at launch
+  static constexpr int kLaunchRegs = k8 ? 128 : 168;
+  static constexpr int kUtil = k8 ? 48 : 88;
+  static constexpr int kConvert = 80;
+  static constexpr int kSoftmax = k8 ? 192 : 208;
+  static constexpr int kBlockRegs = 128 * kUtil + 256 * kSoftmax + (k8 ? 128 * kConvert : 0);
+  static_assert(kBlockRegs <= kThreads * kLaunchRegs, "setmaxnreg would wait for ever");
+  static_assert(kSmem <= 231424 + 1024, "shared memory of an SM");
+};
+
+struct RowsParams {
+  Segment s;
+  RowShape q;
+  int tile_b, tile_pos;   // sequences and positions of a query tile: its rows are tile_b x tile_pos x group
+  int pos_tiles;          // tiles along the positions (1 where a tile holds whole sequences)
+  int tiles, blocks;      // query tiles of a unit, and the CTAs' one or two of them
+  int parts;
+  float scale_log2;
+  Partials mine;
+  uint32_t* status;
+};
+
+struct RowsMaps {
+  CUtensorMap q, k, v, ks, vs;
+};
+
+struct Bars {
+  uint64_t q_full[2];
+  uint64_t k_full[3], k_empty[3];
+  uint64_t v_full[3], v_empty[3];
+  uint64_t raw_full[3], raw_empty[3];
+  uint64_t s_full[2], s_free, p_ready[2], pv_done[2];
+};
+
+__device__ __forceinline__ void st_global_v8(void* ptr, const uint32_t* r) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(ptr), "r"(r[0]), "r"(r[1]),
+               "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+               : "memory");
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float y;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
+  return y;
+}
+__device__ __forceinline__ void lds4(uint32_t addr, uint32_t* r) {
+  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void sts4(uint32_t addr, const uint32_t* r) {
+  asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]) : "memory");
+}
+__device__ __forceinline__ float ldsf(uint32_t addr) {
+  float v;
+  asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+  return v;
+}
+__device__ __forceinline__ void record_timeout(uint32_t* status, uint32_t site) {
+  atomicAdd(&status[0], 1u);
+  status[1] = site;
+}
+
+// Four codes times their scale, in q's type.
+template <bool kBF16, int kFmt>
+__device__ __forceinline__ void restore4(uint32_t w, float2 scale, uint32_t& lo, uint32_t& hi) {
+  uint32_t a, b;
+  codes_to_f16<kFmt>(w, a, b);
+  const float2 x = __fmul2_rn(unpack2<false>(a), scale), y = __fmul2_rn(unpack2<false>(b), scale);
+  lo = pack2<kBF16>(x.x, x.y);
+  hi = pack2<kBF16>(y.x, y.y);
+}
+
+// Grid: parts of the keys x blocks of query tiles x units, the blocks of a part side by side (they read the same keys).
+template <bool kBF16, int kFmt, bool kPair>
+__global__ void __launch_bounds__(Cfg<kFmt, kPair>::kThreads, 1)
+attn_rows_kernel(const __grid_constant__ RowsMaps maps, const RowsParams p) {
+  using C = Cfg<kFmt, kPair>;
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ __align__(8) Bars bars;
+  __shared__ float2 row_s[kPair ? 1 : kTile];  // (one tile) second slot's reference and sum; then both slots' factors
+  __shared__ uint32_t tmem_base_s;
+  __shared__ uint32_t abort_s;
+
+  const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  const uint32_t sQ = smem_base, sK = sQ + C::kQ * kTileBytes, sV = sK + C::kK * kTileBytes;
+  const uint32_t sRaw = sV + C::kV * kTileBytes, sScale = sRaw + C::kRaw * kRawBytes;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  volatile uint32_t* abortp = &abort_s;
+
+  int x = static_cast<int>(blockIdx.x);
+  const int block = x % p.blocks;
+  x /= p.blocks;
+  const int part = x % p.parts, unit = x / p.parts;
+  const int seq = unit / p.q.Hkv, hk = unit % p.q.Hkv;
+  const int tile0 = kPair ? 2 * block : block;
+  const bool two = kPair && tile0 + 1 < p.tiles;
+
+  if (tid == 0) {
+    abort_s = 0;
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(smem_u32(&bars.q_full[i]), 1);
+      mbar_init(smem_u32(&bars.s_full[i]), 1);
+      mbar_init(smem_u32(&bars.p_ready[i]), 128);
+      mbar_init(smem_u32(&bars.pv_done[i]), 1);
+    }
+    mbar_init(smem_u32(&bars.s_free), 128);
+    for (int i = 0; i < 3; ++i) {
+      mbar_init(smem_u32(&bars.k_full[i]), C::k8 ? 128 : 1);
+      mbar_init(smem_u32(&bars.k_empty[i]), 1);
+      mbar_init(smem_u32(&bars.v_full[i]), C::k8 ? 128 : 1);
+      mbar_init(smem_u32(&bars.v_empty[i]), 1);
+      mbar_init(smem_u32(&bars.raw_full[i]), 1);
+      mbar_init(smem_u32(&bars.raw_empty[i]), 4);
+    }
+    mbar_fence_init();
+    tma_prefetch_desc(&maps.q);
+    tma_prefetch_desc(&maps.k);
+    tma_prefetch_desc(&maps.v);
+  }
+  if (warp == 1) {
+    __syncwarp();
+    tmem_alloc(smem_u32(&tmem_base_s), 512);
+    tmem_relinquish();
+  }
+  tc_fence_before_sync();
+  __syncthreads();
+  tc_fence_after_sync();
+  const uint32_t tbase = tmem_base_s;
+  griddep_wait();
+  griddep_launch_dependents();
+
+  // This CTA's key tiles: its part of what the sequence has, and of what the block's last rows see.
+  const int len = seen_of(p.s, seq);
+  int limit = len;
+  if (p.s.causal) {
+    const int last = min(tile0 + (two ? 1 : 0), p.tiles - 1) % p.pos_tiles;
+    const int last_pos = p.pos_tiles == 1 || two ? p.q.Sq - 1 : min((last + 1) * p.tile_pos, p.q.Sq) - 1;
+    limit = max(0, min(len, last_pos + len - p.q.Sq + 1));
+  }
+  const int all = (limit + kTile - 1) / kTile;
+  const int j0 = static_cast<int>(static_cast<int64_t>(all) * part / p.parts);
+  const int n = static_cast<int>(static_cast<int64_t>(all) * (part + 1) / p.parts) - j0;
+  const int n0 = kPair ? n : (n + 1) / 2;            // steps of either slot
+  const int n1 = kPair ? (two ? n : 0) : n / 2;
+
+  auto wait_all = [&](uint64_t* bar, uint32_t parity, uint32_t site) -> bool {
+    const bool good = __all_sync(0xffffffffu, mbar_wait(smem_u32(bar), parity, abortp));
+    if (!good && lane == 0) record_timeout(p.status, site);
+    return good;
+  };
+
+  if (warp == 0) {
+    // ------------------------------------------------------------------ TMA: Q, then K or codes
+    reg_dealloc<C::kUtil>();
+    if (lane == 0 && n > 0) {
+      const uint32_t q_bytes = static_cast<uint32_t>(p.tile_b * p.tile_pos * p.q.group) * 128u;  // of a half
+      for (int t = 0; t < (two ? 2 : 1); ++t) {
+        const int tile = tile0 + t;
+        const int b = seq * p.s.n + (p.pos_tiles == 1 ? tile * p.tile_b : tile / p.pos_tiles);
+        const int pos = p.pos_tiles == 1 ? 0 : tile % p.pos_tiles * p.tile_pos;
+        const uint32_t bar = smem_u32(&bars.q_full[t]);
+        mbar_expect_tx(bar, 2 * q_bytes);
+        tma_load_4d(sQ + t * kTileBytes, &maps.q, bar, 0, hk * p.q.group, pos, b);
+        tma_load_4d(sQ + t * kTileBytes + kHalfBytes, &maps.q, bar, 64, hk * p.q.group, pos, b);
+      }
+      if constexpr (C::k8) {
+        bool ok = true;
+        int c = 0;
+        for (; c < 2 * n; ++c) {  // K and V in turn
+          const int st = c % C::kRaw, use = c / C::kRaw, key = (j0 + c / 2) * kTile;
+          if (use > 0 && !mbar_wait(smem_u32(&bars.raw_empty[st]), (use - 1) & 1, abortp)) {
+            record_timeout(p.status, 91);
+            ok = false;
+            break;
+          }
+          if (use > 0) fence_proxy_async_smem();  // (the consumers' reads, behind the wait above, before the copy)
+          const uint32_t bar = smem_u32(&bars.raw_full[st]);
+          mbar_expect_tx(bar, kRawBytes + 512);
+          tma_load_4d(sRaw + st * kRawBytes, (c & 1) ? &maps.v : &maps.k, bar, 0, hk, key, seq);
+          tma_load_4d(sScale + st * 512, (c & 1) ? &maps.vs : &maps.ks, bar, key, hk, seq, 0);
+        }
+        if (!ok) {
+          // give copies already in flight a bounded chance to land before the CTA retires
+          volatile uint32_t none = 0;
+          for (int i = c > C::kRaw ? c - C::kRaw : 0; i < c; ++i)
+            mbar_wait(smem_u32(&bars.raw_full[i % C::kRaw]), (i / C::kRaw) & 1, &none);
+        }
+      } else {
+        bool ok = true;
+        int c = 0;
+        for (; c < n; ++c) {
+          const int st = c % C::kK, use = c / C::kK;
+          if (use > 0 && !mbar_wait(smem_u32(&bars.k_empty[st]), (use - 1) & 1, abortp)) {
+            record_timeout(p.status, 92);
+            ok = false;
+            break;
+          }
+          const uint32_t bar = smem_u32(&bars.k_full[st]);
+          mbar_expect_tx(bar, kTileBytes);
+          tma_load_4d(sK + st * kTileBytes, &maps.k, bar, 0, hk, (j0 + c) * kTile, seq);
+          tma_load_4d(sK + st * kTileBytes + kHalfBytes, &maps.k, bar, 64, hk, (j0 + c) * kTile, seq);
+        }
+        if (!ok) {
+          volatile uint32_t none = 0;
+          for (int i = c > C::kK ? c - C::kK : 0; i < c; ++i)
+            mbar_wait(smem_u32(&bars.k_full[i % C::kK]), (i / C::kK) & 1, &none);
+        }
+      }
+    }
+  } else if (warp == 2) {
+    // ------------------------------------------------------------------ TMA: V
+    reg_dealloc<C::kUtil>();
+    if (!C::k8 && lane == 0) {
+      bool ok = true;
+      int c = 0;
+      for (; c < n; ++c) {
+        const int st = c % C::kV, use = c / C::kV;
+        if (use > 0 && !mbar_wait(smem_u32(&bars.v_empty[st]), (use - 1) & 1, abortp)) {
+          record_timeout(p.status, 93);
+          ok = false;
+          break;
+        }
+        const uint32_t bar = smem_u32(&bars.v_full[st]);
+        mbar_expect_tx(bar, kTileBytes);
+        tma_load_4d(sV + st * kTileBytes, &maps.v, bar, 0, hk, (j0 + c) * kTile, seq);
+        tma_load_4d(sV + st * kTileBytes + kHalfBytes, &maps.v, bar, 64, hk, (j0 + c) * kTile, seq);
+      }
+      if (!ok) {
+        volatile uint32_t none = 0;
+        for (int i = c > C::kV ? c - C::kV : 0; i < c; ++i)
+          mbar_wait(smem_u32(&bars.v_full[i % C::kV]), (i / C::kV) & 1, &none);
+      }
+    }
+  } else if (warp == 1) {
+    // ------------------------------------------------------------------ QK^T issuer
+    // Step j of slot 0, step j of slot 1, step j + 1 of slot 0, ...: each when the softmax warps have the one before
+    // it in registers.
+    reg_dealloc<C::kUtil>();
+    constexpr uint32_t kFmtBits = kBF16 ? UMMA_BF16 : UMMA_F16;
+    constexpr uint32_t idesc = umma_idesc_f16(kFmtBits, UMMA_K_MAJOR, UMMA_K_MAJOR, 128, 128);
+    bool ok = true;
+    uint32_t uses = 0;  // of S so far
+    for (int j = 0; j < n0 && ok; ++j) {
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        if (j >= (t ? n1 : n0)) continue;
+        const int c = kPair ? j : 2 * j + t, st = c % C::kK;
+        const bool k_hit = mbar_try_wait(smem_u32(&bars.k_full[st]), (c / C::kK) & 1);
+        const bool s_hit = uses == 0 || mbar_try_wait(smem_u32(&bars.s_free), (uses - 1) & 1);
+        if (j == 0 && (kPair || t == 0)) ok = wait_all(&bars.q_full[t], 0, 94);
+        if (ok && !__all_sync(0xffffffffu, k_hit)) ok = wait_all(&bars.k_full[st], (c / C::kK) & 1, 95);
+        if (ok && !__all_sync(0xffffffffu, s_hit)) ok = wait_all(&bars.s_free, (uses - 1) & 1, 96);
+        if (!ok) break;
+        ++uses;
+        tc_fence_after_sync();
+        if (elect_one()) {
+          const uint64_t kdesc = umma_smem_desc_sw128(sK + st * kTileBytes, 16, 1024);
+          const uint64_t qdesc = umma_smem_desc_sw128(sQ + (kPair ? t : 0) * kTileBytes, 16, 1024);
+#pragma unroll
+          for (int kk = 0; kk < 8; ++kk) {
+            const uint64_t off = static_cast<uint64_t>((kk & 3) * 2 + (kk >> 2) * (kHalfBytes >> 4));
+            umma_ss(tbase, qdesc + off, kdesc + off, idesc, kk > 0 ? 1u : 0u);
+          }
+          umma_commit(smem_u32(&bars.s_full[t]));
+          // the K stage is free after the last QK^T that reads it
+          if (!kPair || t == 1 || !two) umma_commit(smem_u32(&bars.k_empty[st]));
+        }
+        __syncwarp();
+      }
+    }
+  } else if (warp == 3) {
+    // ------------------------------------------------------------------ P.V issuer
+    reg_dealloc<C::kUtil>();
+    constexpr uint32_t kFmtBits = kBF16 ? UMMA_BF16 : UMMA_F16;
+    constexpr uint32_t idesc = umma_idesc_f16(kFmtBits, UMMA_K_MAJOR, UMMA_MN_MAJOR, 128, 128);
+    bool ok = true;
+    int cleared = -1;
+    for (int j = 0; j < n0 && ok; ++j) {
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        if (j >= (t ? n1 : n0)) continue;
+        const int c = kPair ? j : 2 * j + t, st = c % C::kV;
+        ok = wait_all(&bars.v_full[st], (c / C::kV) & 1, 97);
+        if (!ok) break;
+        if (!C::k8 && (j0 + c + 1) * kTile > len && cleared != c) {
+          // what lies behind the sequence may be infinite or NaN, and its weights of 0 would not stop that
+          cleared = c;
+          const int live = len - (j0 + c) * kTile;
+          const uint32_t zero[4] = {0, 0, 0, 0};
+          for (int i = live * 16 + lane; i < kTile * 16; i += 32)
+            sts4(sV + st * kTileBytes + (i & 8) * (kHalfBytes / 8) + (i >> 4) * 128 + (i & 7) * 16, zero);
+          fence_proxy_async_smem();
+          __syncwarp();
+        }
+        ok = wait_all(&bars.p_ready[t], j & 1, 98);
+        if (!ok) break;
+        tc_fence_after_sync();
+        if (elect_one()) {
+          const uint64_t vdesc = umma_smem_desc_sw128(sV + st * kTileBytes, kHalfBytes, 1024);
+          const uint32_t tP = tbase + 128 + t * 64, tO = tbase + 256 + t * 128;
+#pragma unroll
+          for (int kk = 0; kk < 8; ++kk)
+            umma_ts(tO, tP + kk * 8, vdesc + static_cast<uint64_t>(kk * (2048 >> 4)), idesc, (j > 0 || kk > 0) ? 1u : 0u);
+          umma_commit(smem_u32(&bars.pv_done[t]));
+          // the V stage is free after the last P.V that reads it
+          if (!kPair || t == 1 || !two) umma_commit(smem_u32(&bars.v_empty[st]));
+        }
+        __syncwarp();
+      }
+    }
+  } else if (warp >= 12) {
+    // ------------------------------------------------------------------ codes to 16-bit tiles, a row to a thread
+    if constexpr (C::k8) {
+      reg_dealloc<C::kConvert>();
+      const int row = tid - 384;
+      bool ok = true;
+      for (int c = 0; c < 2 * n; ++c) {
+        const int st = c % C::kRaw, j = c >> 1;
+        const bool is_v = c & 1;
+        const int ring = is_v ? C::kV : C::kK, to = j % ring, use = j / ring;
+        ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&bars.raw_full[st]), (c / C::kRaw) & 1, abortp));
+        if (ok && use > 0)
+          ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(is_v ? &bars.v_empty[to] : &bars.k_empty[to]), (use - 1) & 1, abortp));
+        if (!ok) {
+          if (lane == 0) record_timeout(p.status, 99);
+          break;
+        }
+        const uint32_t src = sRaw + st * kRawBytes, dst = (is_v ? sV : sK) + to * kTileBytes;
+        const bool live = (j0 + j) * kTile + row < len;  // (what lies behind the sequence may be anything)
+        const float f = ldsf(sScale + st * 512 + row * 4);
+        const float2 scale = make_float2(f, f);
+#pragma unroll
+        for (int ch = 0; ch < 8; ++ch) {
+          uint32_t w[4], y[8];
+          lds4(src + sw128_offset(row, ch), w);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            restore4<kBF16, kFmt>(w[i], scale, y[2 * i], y[2 * i + 1]);
+            y[2 * i] = live ? y[2 * i] : 0u;
+            y[2 * i + 1] = live ? y[2 * i + 1] : 0u;
+          }
+          const uint32_t half = dst + (ch >> 2) * kHalfBytes;
+          sts4(half + sw128_offset(row, (ch & 3) * 2), y);
+          sts4(half + sw128_offset(row, (ch & 3) * 2 + 1), y + 4);
+        }
+        fence_proxy_async_smem();
+        mbar_arrive(smem_u32(is_v ? &bars.v_full[to] : &bars.k_full[to]));
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&bars.raw_empty[st]));
+      }
+    }
+  } else {
+    // ------------------------------------------------------------------ softmax + epilogue
+    reg_alloc<C::kSoftmax>();
+    const int t = (warp - 4) >> 2;
+    const int wq = warp & 3;                     // TMEM lane quarter this warp may touch
+    const int r_in_tile = wq * 32 + lane;
+    const uint32_t lane_base = static_cast<uint32_t>(wq * 32) << 16;
+    const uint32_t tS = tbase + lane_base;
+    const uint32_t tP = tbase + lane_base + 128 + t * 64;
+    const uint32_t tO = tbase + lane_base + 256 + t * 128;
+    const float mul = p.scale_log2;
+    const int n_t = t ? n1 : n0;
+    // this thread's query row
+    const int tile = tile0 + (kPair ? t : 0);
+    bool live = (!kPair || t == 0 || two) && r_in_tile < p.tile_b * p.tile_pos * p.q.group;
+    int64_t number = 0;
+    int lim = len - 1, min_lim = len - 1;        // last visible key of the row, and the least of the tile's
+    {
+      const int per = p.tile_pos * p.q.group;    // rows of a sequence in the tile
+      const int i = p.pos_tiles == 1 ? tile * p.tile_b + r_in_tile / per : tile / p.pos_tiles;
+      const int first_pos = p.pos_tiles == 1 ? 0 : tile % p.pos_tiles * p.tile_pos;
+      const int pos = first_pos + r_in_tile % per / p.q.group;
+      live = live && i < p.s.n && pos < p.q.Sq;
+      number = (static_cast<int64_t>(seq * p.s.n + i) * p.q.Sq + pos) * p.q.H + hk * p.q.group + r_in_tile % p.q.group;
+      if (p.s.causal) {
+        lim = min(lim, pos + len - p.q.Sq);
+        min_lim = min(min_lim, first_pos + len - p.q.Sq);
+      }
+    }
+    bool ok = true;
+    float m_ref = -INFINITY;             // exponent reference of this row, in log2 units of the scaled logit
+    float l = 0.f;                       // row sum under the current reference
+    for (int j = 0; j < n_t && ok; ++j) {
+      ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&bars.s_full[t]), j & 1, abortp));
+      if (!ok) { if (lane == 0) record_timeout(p.status, 100); break; }
+      tc_fence_after_sync();
+      const int jk = (j0 + (kPair ? j : 2 * j + t)) * kTile;  // first key of this tile
+      const int thr = lim - jk;  // columns > thr of this tile are masked for this row
+      // The whole 128-wide row goes to registers at once, and S to the next QK^T.
+      float e[128];
+      {
+        uint32_t(&u)[128] = *reinterpret_cast<uint32_t(*)[128]>(e);
+        tmem_ld32(tS + 0, *reinterpret_cast<uint32_t(*)[32]>(&u[0]));
+        tmem_ld32(tS + 32, *reinterpret_cast<uint32_t(*)[32]>(&u[32]));
+        tmem_ld32(tS + 64, *reinterpret_cast<uint32_t(*)[32]>(&u[64]));
+        tmem_ld32(tS + 96, *reinterpret_cast<uint32_t(*)[32]>(&u[96]));
+        tmem_wait_ld();
+      }
+      tc_fence_before_sync();
+      mbar_arrive(smem_u32(&bars.s_free));
+      if (jk + kTile - 1 > min_lim) {
+#pragma unroll
+        for (int i = 0; i < 128; ++i) e[i] = (i > thr) ? -INFINITY : e[i];
+      }
+      // The tile's row maximum is the reference of a first tile; a later one only moves the reference up
+      // (and rescales what was accumulated under the old one) when it exceeds it by too much.
+      float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+      for (int i = 0; i < 128; i += 8) {
+        mx4[0] = max3(mx4[0], e[i], e[i + 1]);
+        mx4[1] = max3(mx4[1], e[i + 2], e[i + 3]);
+        mx4[2] = max3(mx4[2], e[i + 4], e[i + 5]);
+        mx4[3] = max3(mx4[3], e[i + 6], e[i + 7]);
+      }
+      const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * mul;
+      if (j == 0) {
+        m_ref = mx;
+      } else {
+        const bool need = live && mx > m_ref + kRescaleLimit;
+        if (__any_sync(0xffffffffu, need)) {
+          float alpha = 1.f;
+          if (need) {
+            alpha = ex2(m_ref - mx);
+            m_ref = mx;
+            l *= alpha;
+          }
+          // O_t is the sum over this slot's earlier tiles, complete with their last P.V
+          ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&bars.pv_done[t]), (j - 1) & 1, abortp));
+          if (!ok) { if (lane == 0) record_timeout(p.status, 101); break; }
+          tc_fence_after_sync();
+#pragma unroll
+          for (int c = 0; c < 8; ++c) {
+            uint32_t o[16];
+            tmem_ld16(tO + c * 16, o);
+            tmem_wait_ld();
+#pragma unroll
+            for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
+            tmem_st16(tO + c * 16, o);
+          }
+          tmem_wait_st();
+        }
+      }
+      // two logits per FMA instruction (packed f32x2); P is packed to 16 bits right away
+      const float ref = m_ref > -INFINITY ? m_ref : 0.f;
+      const float2 mul2 = make_float2(mul, mul), neg_m2 = make_float2(-ref, -ref);
+      float2 ts4[4] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f), make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+      uint32_t pk[64];
+#pragma unroll
+      for (int i = 0; i < 64; ++i) {
+        float2 v = __ffma2_rn(make_float2(e[2 * i], e[2 * i + 1]), mul2, neg_m2);
+        v.x = ex2(v.x);
+        v.y = ex2(v.y);
+        ts4[i & 3] = __fadd2_rn(ts4[i & 3], v);
+        pk[i] = pack2<kBF16>(v.x, v.y);
+      }
+      const float2 ts2 = __fadd2_rn(__fadd2_rn(ts4[0], ts4[1]), __fadd2_rn(ts4[2], ts4[3]));
+      l += ts2.x + ts2.y;
+      if (j > 0) {  // P_t is free when the last P.V has read it
+        ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&bars.pv_done[t]), (j - 1) & 1, abortp));
+        if (!ok) { if (lane == 0) record_timeout(p.status, 101); break; }
+        tc_fence_after_sync();
+      }
+      tmem_st32(tP, *reinterpret_cast<uint32_t(*)[32]>(&pk[0]));
+      tmem_st32(tP + 32, *reinterpret_cast<uint32_t(*)[32]>(&pk[32]));
+      tmem_wait_st();
+      tc_fence_before_sync();
+      mbar_arrive(smem_u32(&bars.p_ready[t]));
+    }
+    if (n_t > 0 && ok) {
+      ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&bars.pv_done[t]), (n_t - 1) & 1, abortp));
+      if (!ok && lane == 0) record_timeout(p.status, 102);
+      tc_fence_after_sync();
+    }
+    // ---- the part's results: unnormalised O, reference, sum
+    if (l == 0.f) m_ref = -INFINITY;                // (nothing seen)
+    else if (!(m_ref > -INFINITY)) m_ref = 0.f;     // (nothing but NaN: the sum)
+    float* orow = p.mine.o + (number * p.mine.parts + part) * 128;
+    float2* ml = reinterpret_cast<float2*>(p.mine.ml) + number * p.mine.parts + part;
+    if constexpr (kPair) {
+      if (live) *ml = make_float2(m_ref, l);
+      if (n_t > 0) {
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          uint32_t o[32];
+          tmem_ld32(tO + c * 32, o);
+          tmem_wait_ld();
+          if (live) {
+#pragma unroll
+            for (int g = 0; g < 4; ++g) st_global_v8(orow + c * 32 + g * 8, &o[g * 8]);
+          }
+        }
+      }
+    } else {
+      // the slots' factors to a common reference; each writes half of the columns
+      // (every softmax warp gets to the barriers, expired waits or not)
+      if (t == 1) row_s[r_in_tile] = make_float2(m_ref, l);
+      tc_fence_before_sync();
+      named_bar_sync(1, 256);
+      float f0, f1;
+      if (t == 0) {
+        const float2 o = row_s[r_in_tile];
+        const float mm = fmaxf(m_ref, o.x);
+        f0 = m_ref > -INFINITY ? ex2(m_ref - mm) : 0.f;
+        f1 = o.x > -INFINITY ? ex2(o.x - mm) : 0.f;
+        row_s[r_in_tile] = make_float2(f0, f1);
+        if (live) *ml = make_float2(mm, fmaf(f1, o.y, f0 * l));
+      }
+      named_bar_sync(1, 256);
+      tc_fence_after_sync();
+      if (t == 1) {
+        f0 = row_s[r_in_tile].x;
+        f1 = row_s[r_in_tile].y;
+      }
+      const uint32_t tA = tbase + lane_base + 256 + t * 64;
+      if (n > 0) {
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          uint32_t o0[32], o1[32];
+          tmem_ld32(tA + c * 32, o0);
+          if (n1 > 0) tmem_ld32(tA + 128 + c * 32, o1);
+          tmem_wait_ld();
+#pragma unroll
+          for (int i = 0; i < 32; ++i) {
+            float y = __uint_as_float(o0[i]) * f0;
+            if (n1 > 0) y = fmaf(__uint_as_float(o1[i]), f1, y);
+            o0[i] = __float_as_uint(y);
+          }
+          if (live) {
+#pragma unroll
+            for (int g = 0; g < 4; ++g) st_global_v8(orow + t * 64 + c * 32 + g * 8, &o0[g * 8]);
+          }
+        }
+      }
+    }
+  }
+
+  tc_fence_before_sync();
+  __syncthreads();
+  if (warp == 1) {
+    __syncwarp();
+    tmem_dealloc(tbase, 512);
+  }
+}
+
+// ---- merge: a warp to a query row, four columns to a lane, parts in order -----------------------------
+constexpr int kMergeWarps = 8;
+struct MergeParams {
+  Partials in[2];
+  uint16_t* out;
+  int64_t o_sb, o_ss, o_sh;
+  float* lse2;
+  int B, Sq, H;
+};
+template <bool kBF16>
+__global__ void __launch_bounds__(kMergeWarps * 32) attn_merge_kernel(const MergeParams p) {
+  const int lane = threadIdx.x & 31;
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * kMergeWarps + (threadIdx.x >> 5);
+  griddep_wait();
+  griddep_launch_dependents();
+  if (row >= static_cast<int64_t>(p.B) * p.Sq * p.H) return;
+  float m = -INFINITY;
+#pragma unroll
+  for (int w = 0; w < 2; ++w)
+    for (int x = lane; x < p.in[w].parts; x += 32) m = fmaxf(m, p.in[w].ml[(row * p.in[w].parts + x) * 2]);
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
+  float l = 0.f;
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+  for (int w = 0; w < 2; ++w) {
+    const int parts = p.in[w].parts;
+    const float2* ml = reinterpret_cast<const float2*>(p.in[w].ml) + row * parts;
+    const float4* o = reinterpret_cast<const float4*>(p.in[w].o + row * parts * 128) + lane;
+#pragma unroll 4
+    for (int x = 0; x < parts; ++x) {
+      const float2 a = ml[x];
+      const float4 v = o[x * 32];
+      if (a.x > -INFINITY) {
+        const float f = ex2(a.x - m);
+        l = fmaf(f, a.y, l);
+        acc.x = fmaf(f, v.x, acc.x);
+        acc.y = fmaf(f, v.y, acc.y);
+        acc.z = fmaf(f, v.z, acc.z);
+        acc.w = fmaf(f, v.w, acc.w);
+      }
+    }
+  }
+  const int h = static_cast<int>(row % p.H), pos = static_cast<int>(row / p.H % p.Sq), b = static_cast<int>(row / p.H / p.Sq);
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  reinterpret_cast<uint2*>(p.out + b * p.o_sb + pos * p.o_ss + h * p.o_sh)[lane] =
+      make_uint2(pack2<kBF16>(acc.x * inv, acc.y * inv), pack2<kBF16>(acc.z * inv, acc.w * inv));
+  if (p.lse2 != nullptr && lane == 0) p.lse2[(static_cast<int64_t>(b) * p.H + h) * p.Sq + pos] = m + log2f(l);
+}
+
+// How the rows of a unit make query tiles: whole sequences where one fits, else stretches of one sequence's positions.
+struct Tiles {
+  int b, pos, pos_tiles, count;
+};
+Tiles tiles_of(const Segment& s, const RowShape& q) {
+  Tiles t;
+  const int64_t per = static_cast<int64_t>(q.Sq) * q.group;
+  if (per <= kTile) {
+    t.b = static_cast<int>(kTile / per);
+    if (t.b > s.n) t.b = s.n;
+    t.pos = q.Sq;
+    t.pos_tiles = 1;
+    t.count = (s.n + t.b - 1) / t.b;
+  } else {
+    t.b = 1;
+    t.pos = kTile / q.group;
+    t.pos_tiles = (q.Sq + t.pos - 1) / t.pos;
+    t.count = s.n * t.pos_tiles;
+  }
+  return t;
+}
+
+template <bool kBF16, int kFmt, bool kPair>
+cudaError_t launch_rows_of(const CacheRows& c, const CacheAttnArgs& a, RowsParams& p, const Tiles& tiles, cudaStream_t stream) {
+  using C = Cfg<kFmt, kPair>;
+  RowsMaps maps;
+  const uint32_t box[4] = {64, static_cast<uint32_t>(p.q.group), static_cast<uint32_t>(tiles.pos), static_cast<uint32_t>(tiles.b)};
+  if (tma_host::make_boxed_map(&maps.q, a.q, kBF16, a.B, a.Sq, a.H, 128, a.q_sb, a.q_ss, a.q_sh, box) ||
+      make_rows_map(&maps.k, c, false, p.q.Hkv, kBF16, kTile) || make_rows_map(&maps.v, c, true, p.q.Hkv, kBF16, kTile))
+    return cudaErrorInvalidValue;
+  if (C::k8) {
+    if (make_scale_map(&maps.ks, c, false, p.q.Hkv, kTile) || make_scale_map(&maps.vs, c, true, p.q.Hkv, kTile))
+      return cudaErrorInvalidValue;
+  } else {
+    maps.ks = maps.vs = maps.k;
+  }
+  const auto kern = attn_rows_kernel<kBF16, kFmt, kPair>;
+  cudaError_t e = ensure_dynamic_smem(reinterpret_cast<const void*>(kern), C::kSmem);
+  if (e != cudaSuccess) return e;
+  e = check_register_budget(reinterpret_cast<const void*>(kern), C::kThreads, C::kBlockRegs);
+  if (e != cudaSuccess) return e;
+  const unsigned grid = static_cast<unsigned>(static_cast<int64_t>(p.s.N) * p.q.Hkv * p.parts * p.blocks);
+  e = launch_dependent(kern, dim3(grid), dim3(C::kThreads), C::kSmem, stream, maps, p);
+  count_launch();
+  return e;
+}
+
+template <bool kBF16, int kFmt>
+cudaError_t launch_rows_fmt(const CacheRows& c, const CacheAttnArgs& a, RowsParams& p, const Tiles& tiles, cudaStream_t stream) {
+  return tiles.count > 1 ? launch_rows_of<kBF16, kFmt, true>(c, a, p, tiles, stream)
+                         : launch_rows_of<kBF16, kFmt, false>(c, a, p, tiles, stream);
+}
+
+}  // namespace
+
+// Parts of the keys: what makes the CTAs' rounds times the length of one least.  A CTA's set-up, first loads and
+// epilogue count as four steps of a tile of keys, with one query tile, whose steps are half as long, as eight.
+int attn_rows_parts(const Segment& s, const RowShape& q, int num_sms) {
+  const Tiles tiles = tiles_of(s, q);
+  const int64_t items = static_cast<int64_t>(s.N) * q.Hkv * ((tiles.count + 1) / 2);
+  const int key_tiles = (s.S + kTile - 1) / kTile, fixed = tiles.count > 1 ? 4 : 8;
+  int best = 1;
+  int64_t least = INT64_MAX;
+  for (int parts = 1; parts <= key_tiles && parts <= 64; ++parts) {
+    const int64_t cost = (items * parts + num_sms - 1) / num_sms * ((key_tiles + parts - 1) / parts + fixed);
+    if (cost < least) {
+      least = cost;
+      best = parts;
+    }
+  }
+  return best;
+}
+
+cudaError_t launch_attn_rows(const CacheRows& c, const Segment& s, const CacheAttnArgs& a, const Partials& mine, int,
+                             cudaStream_t stream) {
+  RowsParams p;
+  p.s = s;
+  p.q = RowShape{a.Sq, a.H, a.H / a.group, a.group};
+  const Tiles tiles = tiles_of(s, p.q);
+  p.tile_b = tiles.b;
+  p.tile_pos = tiles.pos;
+  p.pos_tiles = tiles.pos_tiles;
+  p.tiles = tiles.count;
+  p.blocks = (tiles.count + 1) / 2;
+  p.parts = mine.parts;
+  p.scale_log2 = a.softmax_scale * 1.4426950408889634f;
+  p.mine = mine;
+  p.status = device_status_words();
+  if (a.bf16) {
+    if (c.format == CACHE_I8) return launch_rows_fmt<true, CACHE_I8>(c, a, p, tiles, stream);
+    if (c.format == CACHE_E4M3) return launch_rows_fmt<true, CACHE_E4M3>(c, a, p, tiles, stream);
+    return launch_rows_fmt<true, CACHE_16>(c, a, p, tiles, stream);
+  }
+  if (c.format == CACHE_I8) return launch_rows_fmt<false, CACHE_I8>(c, a, p, tiles, stream);
+  if (c.format == CACHE_E4M3) return launch_rows_fmt<false, CACHE_E4M3>(c, a, p, tiles, stream);
+  return launch_rows_fmt<false, CACHE_16>(c, a, p, tiles, stream);
+}
+
+cudaError_t launch_attn_merge(const CacheAttnArgs& a, const Partials& first, const Partials& second, cudaStream_t stream) {
+  MergeParams p;
+  p.in[0] = first;
+  p.in[1] = second;
+  p.out = a.out;
+  p.o_sb = a.o_sb; p.o_ss = a.o_ss; p.o_sh = a.o_sh;
+  p.lse2 = a.lse2;
+  p.B = a.B; p.Sq = a.Sq; p.H = a.H;
+  const int64_t rows = static_cast<int64_t>(a.B) * a.Sq * a.H;
+  const cudaError_t e = launch_dependent(a.bf16 ? attn_merge_kernel<true> : attn_merge_kernel<false>,
+                                         dim3(static_cast<unsigned>((rows + kMergeWarps - 1) / kMergeWarps)),
+                                         dim3(kMergeWarps * 32), 0, stream, p);
+  count_launch();
+  return e;
+}
+
+}  // namespace asuka

@@ -26,6 +26,24 @@ inline encode_tiled_fn get_encode_fn() {
   return fn;
 }
 
+// A [B, S, H, D] tensor of 16-bit elements with arbitrary (element) strides for B, S, H and unit stride for D, in boxes
+// of box[0] = 64 (D) x box[1] (H) x box[2] (S) x box[3] (B) with the 128-byte swizzle.  Out-of-range elements read as zero.
+inline int make_boxed_map(CUtensorMap* map, const void* base, bool is_bf16, int64_t B, int64_t S, int64_t H, int64_t D,
+                          int64_t stride_b, int64_t stride_s, int64_t stride_h, const uint32_t boxes[4]) {
+  encode_tiled_fn fn = get_encode_fn();
+  if (!fn) return -1;
+  cuuint64_t dims[4] = {(cuuint64_t)D, (cuuint64_t)H, (cuuint64_t)S, (cuuint64_t)B};
+  cuuint64_t strides[3] = {(cuuint64_t)stride_h * 2, (cuuint64_t)stride_s * 2,
+                           (cuuint64_t)stride_b * 2};
+  cuuint32_t box[4] = {boxes[0], boxes[1], boxes[2], boxes[3]};
+  cuuint32_t estr[4] = {1, 1, 1, 1};
+  CUresult r = fn(map, is_bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
+                  4, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                  CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? 0 : (int)r;
+}
+
 // A [B, S, H, D] tensor of 16-bit elements with arbitrary (element) strides for B, S, H and unit
 // stride for D, tiled as boxes of 64 (D) x 1 (H) x box_rows (S) x 1 (B) with the 128-byte swizzle:
 // one box lands in shared memory as `box_rows` rows of 128 bytes.  Out-of-range rows read as zero
@@ -33,18 +51,8 @@ inline encode_tiled_fn get_encode_fn() {
 inline int make_bshd_map(CUtensorMap* map, const void* base, bool is_bf16, int64_t B, int64_t S,
                          int64_t H, int64_t D, int64_t stride_b, int64_t stride_s, int64_t stride_h,
                          uint32_t box_rows) {
-  encode_tiled_fn fn = get_encode_fn();
-  if (!fn) return -1;
-  cuuint64_t dims[4] = {(cuuint64_t)D, (cuuint64_t)H, (cuuint64_t)S, (cuuint64_t)B};
-  cuuint64_t strides[3] = {(cuuint64_t)stride_h * 2, (cuuint64_t)stride_s * 2,
-                           (cuuint64_t)stride_b * 2};
-  cuuint32_t box[4] = {64, 1, box_rows, 1};
-  cuuint32_t estr[4] = {1, 1, 1, 1};
-  CUresult r = fn(map, is_bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
-                  4, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                  CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  return r == CUDA_SUCCESS ? 0 : (int)r;
+  const uint32_t box[4] = {64, 1, box_rows, 1};
+  return make_boxed_map(map, base, is_bf16, B, S, H, D, stride_b, stride_s, stride_h, box);
 }
 
 // The same tensor of bytes (8-bit codes): boxes of all 128 columns, so that a row is one swizzled row of 128 bytes.

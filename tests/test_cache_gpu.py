@@ -374,6 +374,18 @@ def test_rows_that_are_not_finite_stay_in_their_sequence(ops, Sq, group, fmt, dt
   assert same(got, clean)
 
 
+@pytest.mark.parametrize("fmt", [None] + FORMATS, ids=str)
+@pytest.mark.parametrize("n, Sq", [(2, 1), (30, 1), (2, 40)])
+def test_a_prefix_of_nothing_but_nan(ops, n, Sq, fmt):
+  # (every part of it has no maximum; the sum still has to say so)
+  prefix, cache = make_cache(2, 300, 2, fmt or torch.float16, 150), make_cache(2 * n, 50, 2, fmt or torch.float16, 151)
+  q = q_of(2 * n, Sq, 4, torch.float16, 152)
+  clean = ops.attn_prefix(q, prefix, cache)
+  (prefix.k if fmt is None else prefix.k_scale)[1].fill_(torch.nan)
+  got = ops.attn_prefix(q, prefix, cache)
+  assert torch.isnan(got[n:]).all() and same(got[:n], clean[:n])
+
+
 @pytest.mark.parametrize("fmt", FORMATS, ids=str)
 @pytest.mark.parametrize("Sq, group", [(1, 4), (30, 2)])
 @pytest.mark.parametrize("spread", [2.0 ** -20, 1.0, 30.0])
