@@ -65,6 +65,28 @@ struct Partials {
   int parts;
 };
 
+// ... or those of a launch that deals the keys out (attn_cache.cu): units are `keys`-key tiles, those of all units numbered
+// through, worker w has tiles share * w .. share * (w + 1) - 1.  A unit in one worker's range has its results under `whole`, by row (or has
+// been finished); of one that begins in a range and goes on behind it the worker's slot 1 has a part, of one that began
+// before it slot 0.
+struct Dealt {
+  int keys;
+  int slot_rows;
+  int64_t* ahead;    // [N] tiles ahead of a sequence's first unit
+  int64_t* share;
+  float* slot_o;     // [workers][2][slot_rows][128]
+  float* slot_ml;    // [workers][2][slot_rows][2]
+  float* whole_o;    // [B * Sq * H][128]
+  float* whole_ml;
+};
+// A segment's partial results, whichever they are.
+struct Source {
+  Segment segment;
+  bool dealt;
+  Partials fixed;  // parts = 0 and not dealt: nothing
+  Dealt deal;
+};
+
 // Codes of four consecutive bytes as f16 pairs: (0, 1) and (2, 3).
 template <int kFmt>
 __device__ __forceinline__ void codes_to_f16(uint32_t w, uint32_t& lo, uint32_t& hi) {
@@ -109,9 +131,10 @@ inline int make_scale_map(CUtensorMap* m, const CacheRows& c, bool values, int H
 
 // attn_rows.cu: a segment of more than 16 rows to a unit leaves its partial results at `mine` (mine.parts of each row)
 int attn_rows_parts(const Segment& s, const RowShape& q, int num_sms);
-cudaError_t launch_attn_rows(const CacheRows& c, const Segment& s, const CacheAttnArgs& a, const Partials& mine, int num_sms,
-                             cudaStream_t stream);
-// ... and the output is what the partial results of up to two segments add up to
-cudaError_t launch_attn_merge(const CacheAttnArgs& a, const Partials& first, const Partials& second, cudaStream_t stream);
+cudaError_t launch_attn_rows(const CacheRows& c, const Segment& s, const CacheAttnArgs& a, const Partials& mine, cudaStream_t stream);
+// ... and the output is what the partial results of up to two segments add up to.  `finished`: units that lay in one range are the
+// output already.
+cudaError_t launch_attn_merge(const CacheAttnArgs& a, const Source& first, const Source& second, bool finished, int workers,
+                              cudaStream_t stream);
 
 }  // namespace asuka

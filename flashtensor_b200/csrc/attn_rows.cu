@@ -581,54 +581,141 @@ attn_rows_kernel(const __grid_constant__ RowsMaps maps, const RowsParams p) {
   }
 }
 
-// ---- merge: a warp to a query row, four columns to a lane, parts in order -----------------------------
-constexpr int kMergeWarps = 8;
+// ---- merge: parts in the order of the keys -------------------------------------------------------------
 struct MergeParams {
-  Partials in[2];
+  Source in[2];
+  bool finished;
+  int workers;
+  RowShape q;
   uint16_t* out;
   int64_t o_sb, o_ss, o_sh;
   float* lse2;
-  int B, Sq, H;
+  int B;
 };
-template <bool kBF16>
-__global__ void __launch_bounds__(kMergeWarps * 32) attn_merge_kernel(const MergeParams p) {
-  const int lane = threadIdx.x & 31;
-  const int64_t row = static_cast<int64_t>(blockIdx.x) * kMergeWarps + (threadIdx.x >> 5);
+// One segment's parts of a row: part i at o + i * 128 * step and ml + i * 2 * step, but the first of a dealt unit where it lies.
+struct Parts {
+  int count;
+  const float* o;
+  const float* ml;
+  int64_t step;         // rows from part to part, from the second one on
+  const float* first_o;
+  const float* first_ml;
+  __device__ __forceinline__ const float* o_at(int i) const { return i == 0 ? first_o : o + i * step * 128; }
+  __device__ __forceinline__ const float2* ml_at(int i) const {
+    return reinterpret_cast<const float2*>(i == 0 ? first_ml : ml + i * step * 2);
+  }
+};
+// (whole: a dealt unit that lay in one range)
+__device__ __forceinline__ Parts parts_of(const Source& f, const RowShape& q, int workers, int b, int pos, int h,
+                                              bool* whole) {
+  Parts x;
+  x.count = 0;
+  *whole = false;
+  const int64_t number = (static_cast<int64_t>(b) * q.Sq + pos) * q.H + h;
+  if (!f.dealt) {
+    x.count = f.fixed.parts;
+    x.first_o = x.o = f.fixed.o + number * f.fixed.parts * 128;
+    x.first_ml = x.ml = f.fixed.ml + number * f.fixed.parts * 2;
+    x.step = 1;
+    return x;
+  }
+  const Dealt& d = f.deal;
+  const int seq = b / f.segment.n, hk = h / q.group;
+  const int tiles = (seen_of(f.segment, seq) + d.keys - 1) / d.keys;
+  if (tiles == 0) return x;
+  const int64_t share = *d.share, begin = d.ahead[seq] + static_cast<int64_t>(hk) * tiles;
+  const int64_t w0 = begin / share, w1 = min((begin + tiles - 1) / share, static_cast<int64_t>(workers - 1));
+  x.count = max(static_cast<int>(w1 - w0) + 1, 0);
+  if (x.count == 1) {
+    *whole = true;
+    x.first_o = x.o = d.whole_o + number * 128;
+    x.first_ml = x.ml = d.whole_ml + number * 2;
+    x.step = 0;
+    return x;
+  }
+  const int r = ((b - seq * f.segment.n) * q.Sq + pos) * q.group + h % q.group;
+  // (a unit that begins with its first worker's range is not ahead of it: slot 1 there, slot 0 behind)
+  const int64_t at = w0 * 2 * d.slot_rows + r;
+  x.o = d.slot_o + at * 128;
+  x.ml = d.slot_ml + at * 2;
+  x.step = 2 * d.slot_rows;
+  x.first_o = x.o + static_cast<int64_t>(d.slot_rows) * 128;
+  x.first_ml = x.ml + static_cast<int64_t>(d.slot_rows) * 2;
+  return x;
+}
+
+// kWarps warps to a query row, each with every kWarps-th part, four columns to a lane.
+constexpr int kMergeThreads = 256;
+template <bool kBF16, int kWarps>
+__global__ void __launch_bounds__(kMergeThreads) attn_merge_kernel(const MergeParams p) {
+  __shared__ float4 acc_s[kWarps > 1 ? kWarps : 1][32];
+  __shared__ float2 ml_s[kWarps > 1 ? kWarps : 1];
+  const int lane = threadIdx.x & 31, w = (threadIdx.x >> 5) % kWarps;
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * (kMergeThreads / 32 / kWarps) + (threadIdx.x >> 5) / kWarps;
   griddep_wait();
   griddep_launch_dependents();
-  if (row >= static_cast<int64_t>(p.B) * p.Sq * p.H) return;
-  float m = -INFINITY;
-#pragma unroll
-  for (int w = 0; w < 2; ++w)
-    for (int x = lane; x < p.in[w].parts; x += 32) m = fmaxf(m, p.in[w].ml[(row * p.in[w].parts + x) * 2]);
-#pragma unroll
-  for (int d = 16; d > 0; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
-  float l = 0.f;
+  if (row >= static_cast<int64_t>(p.B) * p.q.Sq * p.q.H) return;  // (with more warps than one a row is a CTA)
+  const int h = static_cast<int>(row % p.q.H), pos = static_cast<int>(row / p.q.H % p.q.Sq), b = static_cast<int>(row / p.q.H / p.q.Sq);
+  float m = -INFINITY, l = 0.f;
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-  for (int w = 0; w < 2; ++w) {
-    const int parts = p.in[w].parts;
-    const float2* ml = reinterpret_cast<const float2*>(p.in[w].ml) + row * parts;
-    const float4* o = reinterpret_cast<const float4*>(p.in[w].o + row * parts * 128) + lane;
-#pragma unroll 4
-    for (int x = 0; x < parts; ++x) {
-      const float2 a = ml[x];
-      const float4 v = o[x * 32];
-      if (a.x > -INFINITY) {
-        const float f = ex2(a.x - m);
-        l = fmaf(f, a.y, l);
-        acc.x = fmaf(f, v.x, acc.x);
-        acc.y = fmaf(f, v.y, acc.y);
-        acc.z = fmaf(f, v.z, acc.z);
-        acc.w = fmaf(f, v.w, acc.w);
+  for (int x = 0; x < 2; ++x) {
+    if (!p.in[x].dealt && p.in[x].fixed.parts == 0) continue;
+    bool whole;
+    const Parts s = parts_of(p.in[x], p.q, p.workers, b, pos, h, &whole);
+    if (whole && p.finished) return;
+    constexpr int kBatch = 8;
+    for (int i0 = w; i0 < s.count; i0 += kBatch * kWarps) {
+      float2 ml[kBatch];
+      float4 o[kBatch];
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i) {
+        const int part = i0 + i * kWarps;
+        ml[i] = part < s.count ? *s.ml_at(part) : make_float2(-INFINITY, 0.f);
+        if (part < s.count) o[i] = reinterpret_cast<const float4*>(s.o_at(part))[lane];
+      }
+      float top = m;
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i) top = fmaxf(top, ml[i].x);
+      const float down = m > -INFINITY ? ex2(m - top) : 0.f;
+      m = top;
+      l *= down;
+      acc = make_float4(acc.x * down, acc.y * down, acc.z * down, acc.w * down);
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i) {
+        if (ml[i].x > -INFINITY) {  // (a part that saw nothing has left nothing)
+          const float f = ex2(ml[i].x - m);
+          l = fmaf(f, ml[i].y, l);
+          acc.x = fmaf(f, o[i].x, acc.x);
+          acc.y = fmaf(f, o[i].y, acc.y);
+          acc.z = fmaf(f, o[i].z, acc.z);
+          acc.w = fmaf(f, o[i].w, acc.w);
+        }
       }
     }
   }
-  const int h = static_cast<int>(row % p.H), pos = static_cast<int>(row / p.H % p.Sq), b = static_cast<int>(row / p.H / p.Sq);
+  if constexpr (kWarps > 1) {
+    acc_s[w][lane] = acc;
+    if (lane == 0) ml_s[w] = make_float2(m, l);
+    __syncthreads();
+    if (w != 0) return;
+    for (int x = 0; x < kWarps; ++x) m = fmaxf(m, ml_s[x].x);
+    l = 0.f;
+    acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int x = 0; x < kWarps; ++x) {
+      const float2 ml = ml_s[x];
+      if (ml.x > -INFINITY) {
+        const float4 o = acc_s[x][lane];
+        const float f = ex2(ml.x - m);
+        l = fmaf(f, ml.y, l);
+        acc = make_float4(fmaf(f, o.x, acc.x), fmaf(f, o.y, acc.y), fmaf(f, o.z, acc.z), fmaf(f, o.w, acc.w));
+      }
+    }
+  }
   const float inv = l == 0.f ? 0.f : 1.f / l;
   reinterpret_cast<uint2*>(p.out + b * p.o_sb + pos * p.o_ss + h * p.o_sh)[lane] =
       make_uint2(pack2<kBF16>(acc.x * inv, acc.y * inv), pack2<kBF16>(acc.z * inv, acc.w * inv));
-  if (p.lse2 != nullptr && lane == 0) p.lse2[(static_cast<int64_t>(b) * p.H + h) * p.Sq + pos] = m + log2f(l);
+  if (p.lse2 != nullptr && lane == 0) p.lse2[(static_cast<int64_t>(b) * p.q.H + h) * p.q.Sq + pos] = m + log2f(l);
 }
 
 // How the rows of a unit make query tiles: whole sequences where one fits, else stretches of one sequence's positions.
@@ -704,7 +791,7 @@ int attn_rows_parts(const Segment& s, const RowShape& q, int num_sms) {
   return best;
 }
 
-cudaError_t launch_attn_rows(const CacheRows& c, const Segment& s, const CacheAttnArgs& a, const Partials& mine, int,
+cudaError_t launch_attn_rows(const CacheRows& c, const Segment& s, const CacheAttnArgs& a, const Partials& mine,
                              cudaStream_t stream) {
   RowsParams p;
   p.s = s;
@@ -729,18 +816,35 @@ cudaError_t launch_attn_rows(const CacheRows& c, const Segment& s, const CacheAt
   return launch_rows_fmt<false, CACHE_16>(c, a, p, tiles, stream);
 }
 
-cudaError_t launch_attn_merge(const CacheAttnArgs& a, const Partials& first, const Partials& second, cudaStream_t stream) {
+cudaError_t launch_attn_merge(const CacheAttnArgs& a, const Source& first, const Source& second, bool finished, int workers,
+                              cudaStream_t stream) {
   MergeParams p;
   p.in[0] = first;
   p.in[1] = second;
+  p.finished = finished;
+  p.workers = workers;
+  p.q = RowShape{a.Sq, a.H, a.H / a.group, a.group};
   p.out = a.out;
   p.o_sb = a.o_sb; p.o_ss = a.o_ss; p.o_sh = a.o_sh;
   p.lse2 = a.lse2;
-  p.B = a.B; p.Sq = a.Sq; p.H = a.H;
-  const int64_t rows = static_cast<int64_t>(a.B) * a.Sq * a.H;
-  const cudaError_t e = launch_dependent(a.bf16 ? attn_merge_kernel<true> : attn_merge_kernel<false>,
-                                         dim3(static_cast<unsigned>((rows + kMergeWarps - 1) / kMergeWarps)),
-                                         dim3(kMergeWarps * 32), 0, stream, p);
+  p.B = a.B;
+  // Parts of a row: as many as it is given, or as workers share a unit.  A warp has eight in flight.
+  int64_t parts = 0;
+  for (const Source* f : {&first, &second}) {
+    if (f->dealt) {
+      const int64_t tiles = (f->segment.S + f->deal.keys - 1) / f->deal.keys, units = static_cast<int64_t>(f->segment.N) * p.q.Hkv;
+      const int64_t shared = workers / units + 2;
+      parts += shared < tiles ? shared : tiles;
+    } else {
+      parts += f->fixed.parts;
+    }
+  }
+  const bool wide = parts > 16;
+  const int64_t rows = static_cast<int64_t>(a.B) * a.Sq * a.H, per_cta = wide ? 1 : kMergeThreads / 32;
+  const auto kern = a.bf16 ? (wide ? attn_merge_kernel<true, 8> : attn_merge_kernel<true, 1>)
+                           : (wide ? attn_merge_kernel<false, 8> : attn_merge_kernel<false, 1>);
+  const cudaError_t e = launch_dependent(kern, dim3(static_cast<unsigned>((rows + per_cta - 1) / per_cta)), dim3(kMergeThreads),
+                                         0, stream, p);
   count_launch();
   return e;
 }
