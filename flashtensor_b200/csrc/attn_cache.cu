@@ -157,16 +157,6 @@ attn_stream_kernel(const __grid_constant__ StreamMaps maps, const StreamParams p
   ahead_s[tid] = before + upto - mine;
   const int64_t workers = static_cast<int64_t>(gridDim.x) * kWarps;
   const int64_t share = max((total + workers - 1) / workers, static_cast<int64_t>(kMinTiles));
-  if (blockIdx.x == 0) {  // (for the merge)
-    int64_t a = ahead_s[tid];
-    for (int i = tid * per; i < min(n_seqs, (tid + 1) * per); ++i) {
-      Cursor c;
-      at(i, c);
-      p.deal[c.seg].ahead[c.seq] = a;
-      a += static_cast<int64_t>(c.tiles) * p.q.Hkv;
-    }
-    if (tid == 0) *p.deal[0].share = share;
-  }
   __syncthreads();
 
   // (neighbours in the numbering on different SMs, so that a small launch uses all of them)
@@ -292,6 +282,11 @@ attn_stream_kernel(const __grid_constant__ StreamMaps maps, const StreamParams p
         }
       }
       min_lim = s.causal ? min(c.len - 1, c.len - p.q.Sq) : c.len - 1;
+      if (first == 0 && lane == 0) {
+        const int rest = c.tiles - (count - n);  // behind this worker's range
+        p.deal[c.seg].workers[static_cast<int64_t>(c.seq) * p.q.Hkv + c.hk] =
+            make_int2(static_cast<int>(worker), static_cast<int>(worker + (rest > 0 ? (rest + share - 1) / share : 0)));
+      }
 #pragma unroll
       for (int i = 0; i < 16; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
     }
@@ -620,14 +615,12 @@ Plan plan_of(const CacheAttnArgs& a, void* ws, int num_sms) {
     }
     Dealt& d = f.deal;
     d.keys = x.c[i]->format == CACHE_16 ? Tile<CACHE_16>::kKeys : Tile<CACHE_I8>::kKeys;
-    d.ahead = w.take<int64_t>(x.s[i].N);
+    d.workers = w.take<int2>(static_cast<size_t>(x.s[i].N) * q.Hkv);
     if (i == 1 && x.together) {
-      d.share = x.from[0].deal.share;
       d.slot_rows = x.from[0].deal.slot_rows;
       d.slot_o = x.from[0].deal.slot_o;
       d.slot_ml = x.from[0].deal.slot_ml;
     } else {
-      d.share = w.take<int64_t>(1);
       d.slot_rows = x.s[i].rows > x.s[1].rows ? x.s[i].rows : x.s[1].rows;
       if (!x.together) d.slot_rows = x.s[i].rows;
       d.slot_o = w.take<float>(workers * 2 * d.slot_rows * 128);

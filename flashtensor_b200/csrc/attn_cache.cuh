@@ -66,14 +66,13 @@ struct Partials {
 };
 
 // ... or those of a launch that deals the keys out (attn_cache.cu): units are `keys`-key tiles, those of all units numbered
-// through, worker w has tiles share * w .. share * (w + 1) - 1.  A unit in one worker's range has its results under `whole`, by row (or has
-// been finished); of one that begins in a range and goes on behind it the worker's slot 1 has a part, of one that began
-// before it slot 0.
+// through, and every worker has an equal range of them.  A unit in one worker's range has its results under `whole`, by row (or
+// has been finished); of one that begins in a range and goes on behind it the worker's slot 1 has a part, of one that
+// began before it slot 0.
 struct Dealt {
   int keys;
   int slot_rows;
-  int64_t* ahead;    // [N] tiles ahead of a sequence's first unit
-  int64_t* share;
+  int2* workers;     // [N * Hkv] first and last worker of a unit (not written for one without keys)
   float* slot_o;     // [workers][2][slot_rows][128]
   float* slot_ml;    // [workers][2][slot_rows][2]
   float* whole_o;    // [B * Sq * H][128]

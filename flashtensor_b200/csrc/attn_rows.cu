@@ -582,6 +582,7 @@ attn_rows_kernel(const __grid_constant__ RowsMaps maps, const RowsParams p) {
 }
 
 // ---- merge: parts in the order of the keys -------------------------------------------------------------
+// Bound by latency: first what says where the parts lie, for both segments at once, then the parts, up to kBatch of a warp in flight.
 struct MergeParams {
   Source in[2];
   bool finished;
@@ -592,55 +593,38 @@ struct MergeParams {
   float* lse2;
   int B;
 };
-// One segment's parts of a row: part i at o + i * 128 * step and ml + i * 2 * step, but the first of a dealt unit where it lies.
+// One segment's parts of a row: the first, and the others `step` rows from one to the next.
 struct Parts {
   int count;
-  const float* o;
-  const float* ml;
-  int64_t step;         // rows from part to part, from the second one on
   const float* first_o;
   const float* first_ml;
-  __device__ __forceinline__ const float* o_at(int i) const { return i == 0 ? first_o : o + i * step * 128; }
-  __device__ __forceinline__ const float2* ml_at(int i) const {
-    return reinterpret_cast<const float2*>(i == 0 ? first_ml : ml + i * step * 2);
-  }
+  const float* o;
+  const float* ml;
+  int64_t step;
 };
-// (whole: a dealt unit that lay in one range)
-__device__ __forceinline__ Parts parts_of(const Source& f, const RowShape& q, int workers, int b, int pos, int h,
-                                              bool* whole) {
+__device__ __forceinline__ Parts parts_of(const Source& f, const RowShape& q, int workers, int row, int b, int pos, int h) {
   Parts x;
-  x.count = 0;
-  *whole = false;
-  const int64_t number = (static_cast<int64_t>(b) * q.Sq + pos) * q.H + h;
   if (!f.dealt) {
     x.count = f.fixed.parts;
-    x.first_o = x.o = f.fixed.o + number * f.fixed.parts * 128;
-    x.first_ml = x.ml = f.fixed.ml + number * f.fixed.parts * 2;
+    x.first_o = f.fixed.o + static_cast<int64_t>(row) * x.count * 128;
+    x.first_ml = f.fixed.ml + static_cast<int64_t>(row) * x.count * 2;
+    x.o = x.first_o;
+    x.ml = x.first_ml;
     x.step = 1;
     return x;
   }
   const Dealt& d = f.deal;
-  const int seq = b / f.segment.n, hk = h / q.group;
-  const int tiles = (seen_of(f.segment, seq) + d.keys - 1) / d.keys;
-  if (tiles == 0) return x;
-  const int64_t share = *d.share, begin = d.ahead[seq] + static_cast<int64_t>(hk) * tiles;
-  const int64_t w0 = begin / share, w1 = min((begin + tiles - 1) / share, static_cast<int64_t>(workers - 1));
-  x.count = max(static_cast<int>(w1 - w0) + 1, 0);
-  if (x.count == 1) {
-    *whole = true;
-    x.first_o = x.o = d.whole_o + number * 128;
-    x.first_ml = x.ml = d.whole_ml + number * 2;
-    x.step = 0;
-    return x;
-  }
+  const int seq = b / f.segment.n;
+  const int2 w = d.workers[static_cast<int64_t>(seq) * q.Hkv + h / q.group];
+  const bool some = seen_of(f.segment, seq) > 0;
+  x.count = some ? min(max(w.y - w.x, 0) + 1, workers) : 0;  // (bounded, should another stream have changed the length)
   const int r = ((b - seq * f.segment.n) * q.Sq + pos) * q.group + h % q.group;
-  // (a unit that begins with its first worker's range is not ahead of it: slot 1 there, slot 0 behind)
-  const int64_t at = w0 * 2 * d.slot_rows + r;
-  x.o = d.slot_o + at * 128;
+  const int64_t at = static_cast<int64_t>(min(max(w.x, 0), workers - x.count)) * 2 * d.slot_rows + r;
+  x.o = d.slot_o + at * 128;    // slot 0, of all workers but the first
   x.ml = d.slot_ml + at * 2;
   x.step = 2 * d.slot_rows;
-  x.first_o = x.o + static_cast<int64_t>(d.slot_rows) * 128;
-  x.first_ml = x.ml + static_cast<int64_t>(d.slot_rows) * 2;
+  x.first_o = x.count == 1 ? d.whole_o + static_cast<int64_t>(row) * 128 : x.o + static_cast<int64_t>(d.slot_rows) * 128;
+  x.first_ml = x.count == 1 ? d.whole_ml + static_cast<int64_t>(row) * 2 : x.ml + static_cast<int64_t>(d.slot_rows) * 2;
   return x;
 }
 
@@ -651,46 +635,50 @@ __global__ void __launch_bounds__(kMergeThreads) attn_merge_kernel(const MergePa
   __shared__ float4 acc_s[kWarps > 1 ? kWarps : 1][32];
   __shared__ float2 ml_s[kWarps > 1 ? kWarps : 1];
   const int lane = threadIdx.x & 31, w = (threadIdx.x >> 5) % kWarps;
-  const int64_t row = static_cast<int64_t>(blockIdx.x) * (kMergeThreads / 32 / kWarps) + (threadIdx.x >> 5) / kWarps;
+  const int row = static_cast<int>(blockIdx.x) * (kMergeThreads / 32 / kWarps) + static_cast<int>(threadIdx.x >> 5) / kWarps;
+  const int h = row % p.q.H, pos = row / p.q.H % p.q.Sq, b = row / p.q.H / p.q.Sq;
   griddep_wait();
   griddep_launch_dependents();
-  if (row >= static_cast<int64_t>(p.B) * p.q.Sq * p.q.H) return;  // (with more warps than one a row is a CTA)
-  const int h = static_cast<int>(row % p.q.H), pos = static_cast<int>(row / p.q.H % p.q.Sq), b = static_cast<int>(row / p.q.H / p.q.Sq);
+  if (b >= p.B) return;  // (with more warps than one a row is a CTA)
+  const Parts x0 = parts_of(p.in[0], p.q, p.workers, row, b, pos, h), x1 = parts_of(p.in[1], p.q, p.workers, row, b, pos, h);
+  if (p.finished && x1.count == 1) return;
+  const int count = x0.count + x1.count;
   float m = -INFINITY, l = 0.f;
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  constexpr int kBatch = 10;
+  for (int i0 = w; i0 < count; i0 += kBatch * kWarps) {
+    float2 ml[kBatch];
+    float4 o[kBatch];
 #pragma unroll
-  for (int x = 0; x < 2; ++x) {
-    if (!p.in[x].dealt && p.in[x].fixed.parts == 0) continue;
-    bool whole;
-    const Parts s = parts_of(p.in[x], p.q, p.workers, b, pos, h, &whole);
-    if (whole && p.finished) return;
-    constexpr int kBatch = 8;
-    for (int i0 = w; i0 < s.count; i0 += kBatch * kWarps) {
-      float2 ml[kBatch];
-      float4 o[kBatch];
-#pragma unroll
-      for (int i = 0; i < kBatch; ++i) {
-        const int part = i0 + i * kWarps;
-        ml[i] = part < s.count ? *s.ml_at(part) : make_float2(-INFINITY, 0.f);
-        if (part < s.count) o[i] = reinterpret_cast<const float4*>(s.o_at(part))[lane];
+    for (int i = 0; i < kBatch; ++i) {
+      const int part = i0 + i * kWarps;
+      ml[i] = make_float2(-INFINITY, 0.f);
+      if (part < count) {
+        const bool second = part >= x0.count;
+        const int y = second ? part - x0.count : part;
+        const int64_t off = y * (second ? x1.step : x0.step);
+        const float* at_o = second ? (y == 0 ? x1.first_o : x1.o + off * 128) : (y == 0 ? x0.first_o : x0.o + off * 128);
+        const float* at_ml = second ? (y == 0 ? x1.first_ml : x1.ml + off * 2) : (y == 0 ? x0.first_ml : x0.ml + off * 2);
+        ml[i] = *reinterpret_cast<const float2*>(at_ml);
+        o[i] = reinterpret_cast<const float4*>(at_o)[lane];
       }
-      float top = m;
+    }
+    float top = m;
 #pragma unroll
-      for (int i = 0; i < kBatch; ++i) top = fmaxf(top, ml[i].x);
-      const float down = m > -INFINITY ? ex2(m - top) : 0.f;
-      m = top;
-      l *= down;
-      acc = make_float4(acc.x * down, acc.y * down, acc.z * down, acc.w * down);
+    for (int i = 0; i < kBatch; ++i) top = fmaxf(top, ml[i].x);
+    const float down = m > -INFINITY ? ex2(m - top) : 0.f;
+    m = top;
+    l *= down;
+    acc = make_float4(acc.x * down, acc.y * down, acc.z * down, acc.w * down);
 #pragma unroll
-      for (int i = 0; i < kBatch; ++i) {
-        if (ml[i].x > -INFINITY) {  // (a part that saw nothing has left nothing)
-          const float f = ex2(ml[i].x - m);
-          l = fmaf(f, ml[i].y, l);
-          acc.x = fmaf(f, o[i].x, acc.x);
-          acc.y = fmaf(f, o[i].y, acc.y);
-          acc.z = fmaf(f, o[i].z, acc.z);
-          acc.w = fmaf(f, o[i].w, acc.w);
-        }
+    for (int i = 0; i < kBatch; ++i) {
+      if (ml[i].x > -INFINITY) {  // (a part that saw nothing has left nothing)
+        const float f = ex2(ml[i].x - m);
+        l = fmaf(f, ml[i].y, l);
+        acc.x = fmaf(f, o[i].x, acc.x);
+        acc.y = fmaf(f, o[i].y, acc.y);
+        acc.z = fmaf(f, o[i].z, acc.z);
+        acc.w = fmaf(f, o[i].w, acc.w);
       }
     }
   }
