@@ -12,15 +12,18 @@
 //     numbered through.  Every warp of the launch is a worker with an equal, contiguous range of them, which may begin and end
 //     inside a unit: no SM waits for the longest sequence, and a warp waits for no other;
 //   - a warp fetches its own tiles by TMA into a ring of its own, across the ends of units, and works on them with 16x8x16 matrix
-//     instructions and a running maximum and sum;
+//     instructions and a running maximum and sum.  The keys are the 16 rows of the first product, S^T = K Q^T, and the columns
+//     of the values those of the second, O^T = V^T P^T, so that eight query rows, the usual case, cost half of what sixteen do;
+//     the weights get from one to the other by transposing 8x8 blocks between registers;
 //   - a unit that lies in one range is finished there; what a range has of a unit that others share goes to the workspace
 //     and is merged by attn_merge_kernel in the order of the keys, so results do not depend on which warp was first.
 // Codes of 8 bits go from shared memory straight into matrix fragments:
 //   - codes become f16, exactly (int8 as the low bits of 1024 + 128 + code, less 1152; e4m3 by conversion), and q is brought
 //     to f16 too, a bf16 row times the power of two that puts its largest value in [1, 2): what is lost is below 2^-24 of it;
-//   - the order of a contraction's terms is free: lane l & 3 = t takes columns 32 t .. 32 t + 31 of its keys' rows, 16 bytes at a
-//     time, and the query fragments are loaded in that order; for the second product lane l >> 2 = c takes columns 16 c .. 16 c + 15
-//     of four keys, whose bytes are interleaved to pairs of keys.  With the 128-byte swizzle neither read has a bank conflict;
+//   - the order of a contraction's terms is free, and so is that of a product's rows: lane l & 3 = t takes columns 32 t .. 32 t + 31 of
+//     its keys' rows, 16 bytes at a time, and of its query row; for the second product lane l >> 2 = c takes columns
+//     16 c .. 16 c + 15 of four keys, whose bytes are interleaved to pairs of keys.  With the 128-byte swizzle neither read has a
+//     bank conflict;
 //   - a key's scale multiplies its logits; a value's scale s multiplies the weights, w s = exp2(x) s, rounded to f16.  The reference of
 //     the exponentials is the largest x + log2(s), so w s <= 1 and the rounding is 2^-11 of it (2^-25 of the largest where it is
 //     subnormal).
@@ -74,10 +77,16 @@ __device__ __forceinline__ void ldsm4_t(uint32_t addr, uint32_t (&r)[4]) {
 __device__ __forceinline__ void lds4(uint32_t addr, uint32_t* r) {
   asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
 }
-__device__ __forceinline__ float2 lds2f(uint32_t addr) {
-  float2 v;
-  asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(addr) : "memory");
+__device__ __forceinline__ float ldsf(uint32_t addr) {
+  float v;
+  asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
   return v;
+}
+// an 8x8 block of 16-bit values, rows and columns exchanged
+__device__ __forceinline__ uint32_t transpose8(uint32_t x) {
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
 }
 template <bool kBF16>
 __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
@@ -96,8 +105,8 @@ struct Cursor {
   int len, tiles;  // of the sequence
 };
 
-// One CTA to an SM; a warp is a worker.
-template <bool kBF16, int kFmt>
+// One CTA to an SM; a warp is a worker.  kOct: eights of query rows to a unit.
+template <bool kBF16, int kFmt, int kOct>
 __global__ void __launch_bounds__(kThreads, 1)
 attn_stream_kernel(const __grid_constant__ StreamMaps maps, const StreamParams p) {
   using T = Tile<kFmt>;
@@ -220,13 +229,13 @@ attn_stream_kernel(const __grid_constant__ StreamMaps maps, const StreamParams p
     if (fetched + 1 < count) advance(ahead);
   }
 
-  const int r0 = lane >> 2, t4 = lane & 3;  // query rows of this thread: r0 and r0 + 8 of the unit's 16
-  uint32_t qf[8][4];                        // as matrix fragments (in the order of terms that the keys' have)
-  int lim[2];                               // last visible key of either row
-  int min_lim = 0;                          // no row's is below this
-  float mul[2];                             // of a dot product, to a logit in log2 units
-  float o[16][4], m[2], l[2];               // (l: this thread's columns only)
-  int first = 0;                            // the unit's first tile in this range
+  const int r0 = lane >> 2, t4 = lane & 3;
+  uint32_t qf[kOct][16];      // query row 8 y + r0 as matrix fragments (in the order of terms that the keys' have)
+  int lim[kOct][2];           // last visible key of rows 8 y + 2 t4 and 8 y + 2 t4 + 1, whose logits this thread has
+  int min_lim = 0;            // no row's is below this
+  float mul[kOct][2];         // of a dot product, to a logit in log2 units
+  float o[kOct][8][4], m[kOct][2], l[kOct][2];  // (l: this thread's keys only)
+  int first = 0;              // the unit's first tile in this range
   bool ok = true, begin = true;
 
   for (int n = 0; n < count; ++n) {
@@ -235,35 +244,29 @@ attn_stream_kernel(const __grid_constant__ StreamMaps maps, const StreamParams p
       first = c.tile;
       const Segment& s = p.s[c.seg];
 #pragma unroll
-      for (int x = 0; x < 2; ++x) {
-        const int r = r0 + 8 * x;
+      for (int y = 0; y < kOct; ++y) {
+        const int r = 8 * y + r0;
         const Row row = decode_row(min(r, s.rows - 1), c.seq, c.hk, s, p.q);
-        lim[x] = s.causal ? min(c.len - 1, row.pos + c.len - p.q.Sq) : c.len - 1;
-        mul[x] = p.scale_log2;
-        m[x] = -INFINITY;
-        l[x] = 0.f;
         const uint32_t* src = reinterpret_cast<const uint32_t*>(p.qp + row.b * p.q_sb + row.pos * p.q_ss + row.h * p.q_sh);
         const bool live = r < s.rows;
+        float unit = p.scale_log2;  // of this thread's own row
         if constexpr (!k8) {
 #pragma unroll
-          for (int kk = 0; kk < 8; ++kk) {
-            qf[kk][x] = live ? __ldg(src + t4 + kk * 8) : 0u;
-            qf[kk][2 + x] = live ? __ldg(src + t4 + kk * 8 + 4) : 0u;
-          }
+          for (int kk = 0; kk < 16; ++kk) qf[y][kk] = live ? __ldg(src + t4 + kk * 4) : 0u;
         } else {
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             const uint4 w = live ? __ldg(reinterpret_cast<const uint4*>(src) + t4 * 4 + i) : make_uint4(0, 0, 0, 0);
-            qf[2 * i][x] = w.x;
-            qf[2 * i][2 + x] = w.y;
-            qf[2 * i + 1][x] = w.z;
-            qf[2 * i + 1][2 + x] = w.w;
+            qf[y][4 * i] = w.x;
+            qf[y][4 * i + 1] = w.y;
+            qf[y][4 * i + 2] = w.z;
+            qf[y][4 * i + 3] = w.w;
           }
           if constexpr (kBF16) {
             float top = 0.f;
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
-              const float2 v = unpack2<true>(qf[i >> 1][(i & 1) * 2 + x]);
+              const float2 v = unpack2<true>(qf[y][i]);
               top = fmaxf(top, fmaxf(fabsf(v.x), fabsf(v.y)));
             }
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
@@ -271,15 +274,24 @@ attn_stream_kernel(const __grid_constant__ StreamMaps maps, const StreamParams p
             // (rows of zeros, and of nothing but values under 2^-100, stay as they are or vanish)
             const int e = min(max(static_cast<int>(__float_as_uint(top) >> 23), 27), 253);
             const float down = __uint_as_float(static_cast<uint32_t>(254 - e) << 23);
-            mul[x] *= __uint_as_float(static_cast<uint32_t>(e) << 23);
+            unit *= __uint_as_float(static_cast<uint32_t>(e) << 23);
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
-              uint32_t& w = qf[i >> 1][(i & 1) * 2 + x];
-              const float2 v = unpack2<true>(w);
-              w = pack2<false>(v.x * down, v.y * down);
+              const float2 v = unpack2<true>(qf[y][i]);
+              qf[y][i] = pack2<false>(v.x * down, v.y * down);
             }
           }
         }
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          mul[y][x] = __shfl_sync(0xffffffffu, unit, (2 * t4 + x) * 4);
+          const int pos = min(8 * y + 2 * t4 + x, s.rows - 1) / p.q.group % p.q.Sq;
+          lim[y][x] = s.causal ? min(c.len - 1, pos + c.len - p.q.Sq) : c.len - 1;
+          m[y][x] = -INFINITY;
+          l[y][x] = 0.f;
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) o[y][i][0] = o[y][i][1] = o[y][i][2] = o[y][i][3] = 0.f;
       }
       min_lim = s.causal ? min(c.len - 1, c.len - p.q.Sq) : c.len - 1;
       if (first == 0 && lane == 0) {
@@ -287,8 +299,6 @@ attn_stream_kernel(const __grid_constant__ StreamMaps maps, const StreamParams p
         p.deal[c.seg].workers[static_cast<int64_t>(c.seq) * p.q.Hkv + c.hk] =
             make_int2(static_cast<int>(worker), static_cast<int>(worker + (rest > 0 ? (rest + share - 1) / share : 0)));
       }
-#pragma unroll
-      for (int i = 0; i < 16; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
     }
 
     const int st = n % kStages;
@@ -302,147 +312,170 @@ attn_stream_kernel(const __grid_constant__ StreamMaps maps, const StreamParams p
     }
     const uint32_t sK = ring + st * kTileBytes, sV = sK + T::kK, sKs = scales + st * T::kScales, sVs = sKs + T::kKeys * 4;
     const int key0 = c.tile * T::kKeys;
-    const bool ragged = key0 + T::kKeys > c.len;
-    // s[j][e]: row r0 (e < 2) or r0 + 8, key 8 j + 2 t4 + (e & 1)
-    float s[2 * kSub][4];
+    // s[u][y][e]: key 16 u + r0 (e < 2) or 16 u + 8 + r0, query row 8 y + 2 t4 + (e & 1)
+    float s[kSub][kOct][4];
 #pragma unroll
-    for (int j = 0; j < 2 * kSub; ++j) s[j][0] = s[j][1] = s[j][2] = s[j][3] = 0.f;
-    float2 vs[2 * kSub];
+    for (int u = 0; u < kSub; ++u)
+#pragma unroll
+      for (int y = 0; y < kOct; ++y) s[u][y][0] = s[u][y][1] = s[u][y][2] = s[u][y][3] = 0.f;
+    float ks[2 * kSub], vs[2 * kSub];  // scales of keys 8 j + r0
     if constexpr (k8) {
 #pragma unroll
-      for (int j = 0; j < 2 * kSub; ++j) {
-        uint32_t w[8];
-        lds4(sK + sw128_offset(8 * j + r0, 2 * t4), w);
-        lds4(sK + sw128_offset(8 * j + r0, 2 * t4 + 1), w + 4);
+      for (int u = 0; u < kSub; ++u) {
+        uint32_t a[8], b[8];
+        lds4(sK + sw128_offset(16 * u + r0, 2 * t4), a);
+        lds4(sK + sw128_offset(16 * u + r0, 2 * t4 + 1), a + 4);
+        lds4(sK + sw128_offset(16 * u + 8 + r0, 2 * t4), b);
+        lds4(sK + sw128_offset(16 * u + 8 + r0, 2 * t4 + 1), b + 4);
 #pragma unroll
         for (int kk = 0; kk < 8; ++kk) {
-          uint32_t b0, b1;
-          codes_to_f16<kFmt>(w[kk], b0, b1);
-          mma16816<false>(s[j], qf[kk], b0, b1);
+          uint32_t kf[4];
+          codes_to_f16<kFmt>(a[kk], kf[0], kf[2]);
+          codes_to_f16<kFmt>(b[kk], kf[1], kf[3]);
+#pragma unroll
+          for (int y = 0; y < kOct; ++y) mma16816<false>(s[u][y], kf, qf[y][2 * kk], qf[y][2 * kk + 1]);
         }
       }
 #pragma unroll
       for (int j = 0; j < 2 * kSub; ++j) {
-        const float2 ks = lds2f(sKs + (8 * j + 2 * t4) * 4);
-        vs[j] = lds2f(sVs + (8 * j + 2 * t4) * 4);
-        s[j][0] *= ks.x * mul[0];
-        s[j][1] *= ks.y * mul[0];
-        s[j][2] *= ks.x * mul[1];
-        s[j][3] *= ks.y * mul[1];
+        ks[j] = ldsf(sKs + (8 * j + r0) * 4);
+        vs[j] = ldsf(sVs + (8 * j + r0) * 4);
       }
     } else {
-      // addresses of this lane's rows for the 8x8 blocks: keys of the tile's 16, 16-byte chunk of a row
-      const int k_row = ((lane >> 4) << 3) + (lane & 7), k_chunk = (lane >> 3) & 1;
+      // this lane's row of the 8x8 blocks: keys 0-7 and 8-15, columns 0-7 and 8-15
+      const int k_row = (((lane >> 3) & 1) << 3) + (lane & 7), k_chunk = lane >> 4;
 #pragma unroll
       for (int kk = 0; kk < 8; ++kk) {
-        uint32_t kf[4];  // keys 0-7: k 0-7, 8-15; keys 8-15: k 0-7, 8-15
+        uint32_t kf[4];
         ldsm4(sK + (kk >> 2) * T::kHalf + sw128_offset(k_row, (kk & 3) * 2 + k_chunk), kf);
-        mma16816<kBF16>(s[0], qf[kk], kf[0], kf[1]);
-        mma16816<kBF16>(s[1], qf[kk], kf[2], kf[3]);
+#pragma unroll
+        for (int y = 0; y < kOct; ++y) mma16816<kBF16>(s[0][y], kf, qf[y][2 * kk], qf[y][2 * kk + 1]);
       }
-#pragma unroll
-      for (int j = 0; j < 2; ++j)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) s[j][e] *= mul[0];
     }
-    if (key0 + T::kKeys - 1 > min_lim) {
+    if constexpr (k8) {
 #pragma unroll
-      for (int j = 0; j < 2 * kSub; ++j) {
-        const int key = key0 + 8 * j + 2 * t4;
+      for (int u = 0; u < kSub; ++u)
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (key + (e & 1) > lim[e >> 1]) s[j][e] = -INFINITY;
-        if constexpr (k8) {
-          if (key >= c.len) vs[j].x = 0.f;
-          if (key + 1 >= c.len) vs[j].y = 0.f;
+        for (int y = 0; y < kOct; ++y)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) s[u][y][e] *= ks[2 * u + (e >> 1)] * mul[y][e & 1];
+    } else {
+#pragma unroll
+      for (int y = 0; y < kOct; ++y)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[0][y][e] *= p.scale_log2;
+    }
+    const bool ragged = key0 + T::kKeys - 1 > min_lim;
+    if (ragged) {
+#pragma unroll
+      for (int u = 0; u < kSub; ++u)
+#pragma unroll
+        for (int z = 0; z < 2; ++z) {
+          const int key = key0 + 16 * u + 8 * z + r0;
+#pragma unroll
+          for (int y = 0; y < kOct; ++y)
+#pragma unroll
+            for (int x = 0; x < 2; ++x)
+              if (key > lim[y][x]) s[u][y][2 * z + x] = -INFINITY;
+          if (k8 && key >= c.len) vs[2 * u + z] = 0.f;
         }
-      }
     }
-    float w[2];
+    float w[kOct][2];
+    bool moved = false;
     {
-      float2 lv[2 * kSub];  // log2 of the values' scales
+      float lv[2 * kSub];  // log2 of the values' scales
       if constexpr (k8) {
 #pragma unroll
-        for (int j = 0; j < 2 * kSub; ++j)
-          lv[j] = make_float2(lg2(fmaxf(fabsf(vs[j].x), 0x1p-100f)), lg2(fmaxf(fabsf(vs[j].y), 0x1p-100f)));
+        for (int j = 0; j < 2 * kSub; ++j) lv[j] = lg2(fmaxf(fabsf(vs[j]), 0x1p-100f));
       }
 #pragma unroll
-      for (int x = 0; x < 2; ++x) {
-        float mx = m[x];
+      for (int y = 0; y < kOct; ++y) {
 #pragma unroll
-        for (int j = 0; j < 2 * kSub; ++j) {
-          if constexpr (k8) mx = fmaxf(mx, fmaxf(s[j][2 * x] + lv[j].x, s[j][2 * x + 1] + lv[j].y));
-          else mx = fmaxf(mx, fmaxf(s[j][2 * x], s[j][2 * x + 1]));
-        }
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-        const float ref = mx > -INFINITY ? mx : 0.f;
-        w[x] = ex2(m[x] - ref);
-        m[x] = mx;
-        float sum = 0.f;
+        for (int x = 0; x < 2; ++x) {
+          float mx = m[y][x];
 #pragma unroll
-        for (int j = 0; j < 2 * kSub; ++j) {
-          s[j][2 * x] = ex2(s[j][2 * x] - ref);
-          s[j][2 * x + 1] = ex2(s[j][2 * x + 1] - ref);
-          sum += s[j][2 * x] + s[j][2 * x + 1];
+          for (int j = 0; j < 2 * kSub; ++j) mx = fmaxf(mx, k8 ? s[j >> 1][y][2 * (j & 1) + x] + lv[j] : s[j >> 1][y][2 * (j & 1) + x]);
+          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
+          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+          const float ref = mx > -INFINITY ? mx : 0.f;
+          w[y][x] = ex2(m[y][x] - ref);
+          moved = moved || w[y][x] != 1.f;
+          m[y][x] = mx;
+          float sum = 0.f;
+#pragma unroll
+          for (int j = 0; j < 2 * kSub; ++j) {
+            float& e = s[j >> 1][y][2 * (j & 1) + x];
+            e = ex2(e - ref);
+            sum += e;
+          }
+          l[y][x] = l[y][x] * w[y][x] + sum;
         }
-        l[x] = l[x] * w[x] + sum;
       }
     }
-    if (__any_sync(0xffffffffu, w[0] != 1.f || w[1] != 1.f)) {
+    if (__any_sync(0xffffffffu, moved)) {
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        o[i][0] *= w[0];
-        o[i][1] *= w[0];
-        o[i][2] *= w[1];
-        o[i][3] *= w[1];
-      }
+      for (int y = 0; y < kOct; ++y)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          o[y][i][0] *= w[y][0];
+          o[y][i][1] *= w[y][1];
+          o[y][i][2] *= w[y][0];
+          o[y][i][3] *= w[y][1];
+        }
     }
 #pragma unroll
     for (int u = 0; u < kSub; ++u) {
-      const int kb = 16 * u;  // block of 16 keys
-      uint32_t pf[4];
+      uint32_t pf[kOct][2];  // the weights, rows and keys exchanged: keys 2 t4, 2 t4 + 1 (and 8 further) of row r0
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int j = 2 * u + (e >> 1), x = 2 * (e & 1);
-        if constexpr (k8) pf[e] = pack2<false>(s[j][x] * vs[j].x, s[j][x + 1] * vs[j].y);
-        else pf[e] = pack2<kBF16>(s[j][x], s[j][x + 1]);
-      }
+      for (int y = 0; y < kOct; ++y)
+#pragma unroll
+        for (int z = 0; z < 2; ++z) {
+          const float f = k8 ? vs[2 * u + z] : 1.f;
+          pf[y][z] = transpose8(k8 ? pack2<false>(s[u][y][2 * z] * f, s[u][y][2 * z + 1] * f)
+                                   : pack2<kBF16>(s[u][y][2 * z], s[u][y][2 * z + 1]));
+        }
       if constexpr (k8) {
-        uint32_t v[4][4];  // keys 2 t4, 2 t4 + 1, 8 + 2 t4, 9 + 2 t4 of the block, 16 columns each
+        uint32_t v[4][4];  // keys 2 t4, 2 t4 + 1, 8 + 2 t4, 9 + 2 t4 of the block, columns 16 r0 .. 16 r0 + 15
 #pragma unroll
-        for (int i = 0; i < 4; ++i) lds4(sV + sw128_offset(kb + (i >> 1) * 8 + 2 * t4 + (i & 1), r0), v[i]);
-        if (ragged) {
+        for (int i = 0; i < 4; ++i) lds4(sV + sw128_offset(16 * u + (i >> 1) * 8 + 2 * t4 + (i & 1), r0), v[i]);
+        if (ragged) {  // (what lies behind the sequence may be NaN)
 #pragma unroll
           for (int i = 0; i < 4; ++i)
-            if (key0 + kb + (i >> 1) * 8 + 2 * t4 + (i & 1) >= c.len) v[i][0] = v[i][1] = v[i][2] = v[i][3] = 0u;
+            if (key0 + 16 * u + (i >> 1) * 8 + 2 * t4 + (i & 1) >= c.len) v[i][0] = v[i][1] = v[i][2] = v[i][3] = 0u;
         }
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          uint32_t b0[4], b1[4];  // columns 4 i .. 4 i + 3
-          codes_to_f16<kFmt>(__byte_perm(v[0][i], v[1][i], 0x5140), b0[0], b0[1]);
-          codes_to_f16<kFmt>(__byte_perm(v[0][i], v[1][i], 0x7362), b0[2], b0[3]);
-          codes_to_f16<kFmt>(__byte_perm(v[2][i], v[3][i], 0x5140), b1[0], b1[1]);
-          codes_to_f16<kFmt>(__byte_perm(v[2][i], v[3][i], 0x7362), b1[2], b1[3]);
+          uint32_t vf[2][4];  // columns 4 i, 4 i + 1 and 4 i + 2, 4 i + 3
 #pragma unroll
-          for (int x = 0; x < 4; ++x) mma16816<false>(o[4 * i + x], pf, b0[x], b1[x]);
+          for (int z = 0; z < 2; ++z) {
+            codes_to_f16<kFmt>(__byte_perm(v[2 * z][i], v[2 * z + 1][i], 0x5140), vf[0][2 * z], vf[0][2 * z + 1]);
+            codes_to_f16<kFmt>(__byte_perm(v[2 * z][i], v[2 * z + 1][i], 0x7362), vf[1][2 * z], vf[1][2 * z + 1]);
+          }
+#pragma unroll
+          for (int x = 0; x < 2; ++x)
+#pragma unroll
+            for (int y = 0; y < kOct; ++y) mma16816<false>(o[y][2 * i + x], vf[x], pf[y][0], pf[y][1]);
         }
       } else {
-        const int v_row = kb + (((lane >> 3) & 1) << 3) + (lane & 7), v_chunk = lane >> 4;
+        // 8x8 blocks with rows and columns exchanged: columns 0-7 and 8-15 of keys 0-7, then of keys 8-15
+        const int v_row = ((lane >> 4) << 3) + (lane & 7), v_chunk = (lane >> 3) & 1;
         uint32_t keep[2] = {0xffffffffu, 0xffffffffu};  // (what lies behind the sequence may be infinite or NaN)
         if (ragged) {
 #pragma unroll
-          for (int x = 0; x < 2; ++x) {
-            const int key = key0 + 8 * x + 2 * t4;
-            keep[x] = (key < c.len ? 0xffffu : 0u) | (key + 1 < c.len ? 0xffff0000u : 0u);
+          for (int z = 0; z < 2; ++z) {
+            const int key = key0 + 8 * z + 2 * t4;
+            keep[z] = (key < c.len ? 0xffffu : 0u) | (key + 1 < c.len ? 0xffff0000u : 0u);
           }
         }
 #pragma unroll
         for (int d = 0; d < 8; ++d) {
-          uint32_t vf[4];  // columns 16d + 0-7: keys 0-7, 8-15; columns 16d + 8-15: keys 0-7, 8-15
+          uint32_t vf[4];
           ldsm4_t(sV + (d >> 2) * T::kHalf + sw128_offset(v_row, (d & 3) * 2 + v_chunk), vf);
-          mma16816<kBF16>(o[2 * d], pf, vf[0] & keep[0], vf[1] & keep[1]);
-          mma16816<kBF16>(o[2 * d + 1], pf, vf[2] & keep[0], vf[3] & keep[1]);
+#pragma unroll
+          for (int z = 0; z < 4; ++z) vf[z] &= keep[z >> 1];
+#pragma unroll
+          for (int y = 0; y < kOct; ++y) mma16816<kBF16>(o[y][d], vf, pf[y][0], pf[y][1]);
         }
       }
     }
@@ -458,60 +491,61 @@ attn_stream_kernel(const __grid_constant__ StreamMaps maps, const StreamParams p
 
     if (c.tile + 1 == c.tiles || n + 1 == count) {
       // ---- the unit ends, or this range of it
-#pragma unroll
-      for (int x = 0; x < 2; ++x) {
-        l[x] += __shfl_xor_sync(0xffffffffu, l[x], 1);
-        l[x] += __shfl_xor_sync(0xffffffffu, l[x], 2);
-      }
       const Segment& sg = p.s[c.seg];
       const bool whole = first == 0 && c.tile + 1 == c.tiles;
 #pragma unroll
-      for (int x = 0; x < 2; ++x) {
-        const int r = r0 + 8 * x;
-        if (r >= sg.rows) continue;
-        const Row row = decode_row(r, c.seq, c.hk, sg, p.q);
-        if (whole && p.finish) {
-          const float inv = l[x] == 0.f ? 0.f : 1.f / l[x];
-          uint16_t* dst = p.out + row.b * p.o_sb + row.pos * p.o_ss + row.h * p.o_sh;
-          if constexpr (k8) {  // o[i]: columns 32 t4 + i and 32 t4 + 16 + i
+      for (int y = 0; y < kOct; ++y) {
 #pragma unroll
-            for (int y = 0; y < 2; ++y)
+        for (int x = 0; x < 2; ++x) {
+          float sum = l[y][x];
+          sum += __shfl_xor_sync(0xffffffffu, sum, 4);
+          sum += __shfl_xor_sync(0xffffffffu, sum, 8);
+          sum += __shfl_xor_sync(0xffffffffu, sum, 16);
+          const int r = 8 * y + 2 * t4 + x;
+          if (r >= sg.rows) continue;
+          const Row row = decode_row(r, c.seq, c.hk, sg, p.q);
+          // this thread's columns of the row: 8 bits: 16 r0 + 2 i and + 1 in o[i][x] and o[i][2 + x]; 16 bits: 16 i + r0 and + 8
+          if (whole && p.finish) {
+            const float inv = sum == 0.f ? 0.f : 1.f / sum;
+            uint16_t* dst = p.out + row.b * p.o_sb + row.pos * p.o_ss + row.h * p.o_sh;
+            if constexpr (k8) {
+              uint32_t v[8];
 #pragma unroll
-              for (int i = 0; i < 16; i += 8) {
-                uint32_t v[4];
+              for (int i = 0; i < 8; ++i) v[i] = pack2<kBF16>(o[y][i][x] * inv, o[y][i][2 + x] * inv);
+              *reinterpret_cast<uint4*>(dst + 16 * r0) = make_uint4(v[0], v[1], v[2], v[3]);
+              *reinterpret_cast<uint4*>(dst + 16 * r0 + 8) = make_uint4(v[4], v[5], v[6], v[7]);
+            } else {
 #pragma unroll
-                for (int z = 0; z < 4; ++z)
-                  v[z] = pack2<kBF16>(o[i + 2 * z][2 * x + y] * inv, o[i + 2 * z + 1][2 * x + y] * inv);
-                *reinterpret_cast<uint4*>(dst + 32 * t4 + 16 * y + i) = make_uint4(v[0], v[1], v[2], v[3]);
+              for (int i = 0; i < 8; ++i) {
+                const uint32_t v = pack2<kBF16>(o[y][i][x] * inv, o[y][i][2 + x] * inv);
+                dst[16 * i + r0] = static_cast<uint16_t>(v);
+                dst[16 * i + 8 + r0] = static_cast<uint16_t>(v >> 16);
               }
+            }
+            if (p.lse2 != nullptr && r0 == 0)
+              p.lse2[(static_cast<int64_t>(row.b) * p.q.H + row.h) * p.q.Sq + row.pos] = m[y][x] + log2f(sum);
+            continue;
+          }
+          const Dealt& d = p.deal[c.seg];
+          const int64_t number = (static_cast<int64_t>(row.b) * p.q.Sq + row.pos) * p.q.H + row.h;
+          const int64_t slot = (worker * 2 + (first > 0 ? 0 : 1)) * d.slot_rows + r;
+          float* dst = whole ? d.whole_o + number * 128 : d.slot_o + slot * 128;
+          float* ml = whole ? d.whole_ml + number * 2 : d.slot_ml + slot * 2;
+          if constexpr (k8) {
+#pragma unroll
+            for (int i = 0; i < 8; i += 2)
+              *reinterpret_cast<float4*>(dst + 16 * r0 + 2 * i) = make_float4(o[y][i][x], o[y][i][2 + x], o[y][i + 1][x], o[y][i + 1][2 + x]);
           } else {
 #pragma unroll
-            for (int i = 0; i < 16; ++i)
-              *reinterpret_cast<uint32_t*>(dst + i * 8 + 2 * t4) = pack2<kBF16>(o[i][2 * x] * inv, o[i][2 * x + 1] * inv);
+            for (int i = 0; i < 8; ++i) {
+              dst[16 * i + r0] = o[y][i][x];
+              dst[16 * i + 8 + r0] = o[y][i][2 + x];
+            }
           }
-          if (p.lse2 != nullptr && t4 == 0)
-            p.lse2[(static_cast<int64_t>(row.b) * p.q.H + row.h) * p.q.Sq + row.pos] = m[x] + log2f(l[x]);
-          continue;
-        }
-        const Dealt& d = p.deal[c.seg];
-        const int64_t number = (static_cast<int64_t>(row.b) * p.q.Sq + row.pos) * p.q.H + row.h;
-        const int64_t slot = (worker * 2 + (first > 0 ? 0 : 1)) * d.slot_rows + r;
-        float* dst = whole ? d.whole_o + number * 128 : d.slot_o + slot * 128;
-        float* ml = whole ? d.whole_ml + number * 2 : d.slot_ml + slot * 2;
-        if constexpr (k8) {
-#pragma unroll
-          for (int y = 0; y < 2; ++y)
-#pragma unroll
-            for (int i = 0; i < 16; i += 4)
-              *reinterpret_cast<float4*>(dst + 32 * t4 + 16 * y + i) =
-                  make_float4(o[i][2 * x + y], o[i + 1][2 * x + y], o[i + 2][2 * x + y], o[i + 3][2 * x + y]);
-        } else {
-#pragma unroll
-          for (int i = 0; i < 16; ++i) *reinterpret_cast<float2*>(dst + i * 8 + 2 * t4) = make_float2(o[i][2 * x], o[i][2 * x + 1]);
-        }
-        if (t4 == 0) {
-          const float ref = m[x] > -INFINITY || l[x] == 0.f ? m[x] : 0.f;  // (nothing but NaN: the sum)
-          *reinterpret_cast<float2*>(ml) = make_float2(ref, l[x]);
+          if (r0 == 0) {
+            const float ref = m[y][x] > -INFINITY || sum == 0.f ? m[y][x] : 0.f;  // (nothing but NaN: the sum)
+            *reinterpret_cast<float2*>(ml) = make_float2(ref, sum);
+          }
         }
       }
       begin = true;
@@ -543,7 +577,10 @@ cudaError_t launch_stream_fmt(const CacheRows* const* c, StreamParams& p, bool b
     }
   }
   const uint32_t smem = kWarps * kStages * (kTileBytes + T::kScales) + 1024;
-  const auto kern = bf16 ? attn_stream_kernel<true, kFmt> : attn_stream_kernel<false, kFmt>;
+  bool wide = false;
+  for (int x = 0; x < p.segments; ++x) wide = wide || p.s[x].rows > 8;
+  const auto kern = bf16 ? (wide ? attn_stream_kernel<true, kFmt, 2> : attn_stream_kernel<true, kFmt, 1>)
+                         : (wide ? attn_stream_kernel<false, kFmt, 2> : attn_stream_kernel<false, kFmt, 1>);
   cudaError_t e = ensure_dynamic_smem(reinterpret_cast<const void*>(kern), smem);
   if (e != cudaSuccess) return e;
   e = launch_dependent(kern, dim3(static_cast<unsigned>(num_sms)), dim3(kThreads), smem, stream, maps, p);
