@@ -57,6 +57,7 @@ struct StreamParams {
   int64_t o_sb, o_ss, o_sh;
   float* lse2;
   int finish;      // whole units are the output (no other segment)
+  int chained;     // the kernel ahead is this call's, of the other segment: only the merge needs its results
   Dealt deal[2];
   uint32_t* status;
 };
@@ -131,7 +132,10 @@ attn_stream_kernel(const __grid_constant__ StreamMaps maps, const StreamParams p
       tma_prefetch_desc(&maps.s[x].v);
     }
   }
-  griddep_wait();
+  // Behind this call's own kernel for the prefix the work begins as SMs become free: what this kernel reads was complete
+  // before that one let it start, and what it writes is its own.  (Reads are from L2, and the wait is at the end: the merge follows on
+  // both.)  128 sequences behind 32768 bf16 rows 106.7 -> 101.7 us.
+  if (!p.chained) griddep_wait();
   griddep_launch_dependents();
 
   // ---- the deal: every CTA adds up the tiles of all sequences (a thread has `per` consecutive ones)
@@ -172,7 +176,10 @@ attn_stream_kernel(const __grid_constant__ StreamMaps maps, const StreamParams p
   const int64_t worker = static_cast<int64_t>(warp) * gridDim.x + blockIdx.x;
   const int64_t lo = worker * share;
   const int count = static_cast<int>(min(share, total - lo));  // (a worker's tiles are 8 KB each: far below 2^31)
-  if (count <= 0) return;
+  if (count <= 0) {
+    if (p.chained) griddep_wait();
+    return;
+  }
 
   Cursor c;
   {
@@ -252,11 +259,11 @@ attn_stream_kernel(const __grid_constant__ StreamMaps maps, const StreamParams p
         float unit = p.scale_log2;  // of this thread's own row
         if constexpr (!k8) {
 #pragma unroll
-          for (int kk = 0; kk < 16; ++kk) qf[y][kk] = live ? __ldg(src + t4 + kk * 4) : 0u;
+          for (int kk = 0; kk < 16; ++kk) qf[y][kk] = live ? __ldcg(src + t4 + kk * 4) : 0u;
         } else {
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            const uint4 w = live ? __ldg(reinterpret_cast<const uint4*>(src) + t4 * 4 + i) : make_uint4(0, 0, 0, 0);
+            const uint4 w = live ? __ldcg(reinterpret_cast<const uint4*>(src) + t4 * 4 + i) : make_uint4(0, 0, 0, 0);
             qf[y][4 * i] = w.x;
             qf[y][4 * i + 1] = w.y;
             qf[y][4 * i + 2] = w.z;
@@ -558,6 +565,7 @@ attn_stream_kernel(const __grid_constant__ StreamMaps maps, const StreamParams p
     for (int n = fetched > kStages ? fetched - kStages : 0; n < fetched; ++n)
       mbar_wait(smem_u32(&full[warp][n % kStages]), (n / kStages) & 1, &none);
   }
+  if (p.chained) griddep_wait();
 }
 
 template <int kFmt>
@@ -693,6 +701,7 @@ cudaError_t launch_attn_cache(const CacheAttnArgs& a, void* ws, int num_sms, cud
     cudaError_t e;
     if (x.stream[i]) {
       p.segments = x.together ? 2 : 1;
+      p.chained = i == 1 && x.have[0] ? 1 : 0;
       for (int y = 0; y < p.segments; ++y) {
         p.s[y] = x.s[i + y];
         p.deal[y] = x.from[i + y].deal;

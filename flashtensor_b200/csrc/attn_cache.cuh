@@ -55,7 +55,7 @@ __device__ __forceinline__ Row decode_row(int r, int seq, int hk, const Segment&
   return {seq * s.n + x / q.Sq, x % q.Sq, hk * q.group + g};
 }
 __device__ __forceinline__ int seen_of(const Segment& s, int seq) {
-  return s.len != nullptr ? min(max(s.len[seq], 0), s.S) : s.S;
+  return s.len != nullptr ? min(max(__ldcg(s.len + seq), 0), s.S) : s.S;
 }
 // Partial results of a query row, numbered in the output's own order: `parts` of each, in part order.
 // (A row that saw nothing but NaN has a NaN sum under the reference 0.)
