@@ -14,9 +14,14 @@
 // tile serves both; with one tile a slot has the even key tiles and the other the odd ones, merged at the end.  What is left of a
 // part goes to the workspace unnormalised.
 //
-// 8-bit codes are brought to q's type times their row's scale, rounded once (2^-9 of a value in bf16, 2^-12 in f16, as the
-// cache read back would be): a thread takes one row's 128 codes from the swizzled stage and writes them in the two swizzled halves the
-// tensor pipe reads, neither with a bank conflict.
+// 8-bit codes become f16 tiles in warps of their own: a thread takes one row's 128 codes from the swizzled stage, all at once so that
+// the stage is free again, and writes them times their scale in the two swizzled halves that the tensor pipe reads, neither with a
+// bank conflict.  A code times its scale is rounded once, to f16 (2^-12 on average): the scale, under the power of two of the largest of
+// the warp's 32 keys, is two f16 terms, so that a pair of codes takes two instructions.  The softmax takes the keys'
+// powers of two with the logits' factor; the values' go into the exponent, exp2(x + e - reference), and out of the row sum again.  bf16
+// queries become f16 too, a row times the power of two that puts its largest value in [1, 2).
+// (Scales as f32 in the softmax -- two multiplications and half a shared-memory read for a logit -- took it 4550 clk for a pair of
+// steps instead of 2700; half tiles of codes at a time 5300.)
 #include "attn_cache.cuh"
 
 namespace asuka {
@@ -29,14 +34,19 @@ constexpr uint32_t kHalfBytes = kTileBytes / 2;
 constexpr uint32_t kRawBytes = 128 * 128;       // [128 x 128] codes
 constexpr float kRescaleLimit = 6.0f;           // log2 of the largest exponential tolerated under a stale reference
 
-// kPair: two query tiles; else one.  Shared memory: Q, the rings of 16-bit K and V tiles, of codes, of their scales.
+// kPair: two query tiles; else one.  Shared memory: Q, rings of 16-bit K and V tiles; with 8 bits one ring of both in turn, one of codes,
+// and the scales that come with them.
 template <int kFmt, bool kPair> struct Cfg {
   static constexpr bool k8 = kFmt != CACHE_16;
   static constexpr int kQ = kPair ? 2 : 1;
-  static constexpr int kK = k8 ? 2 : 3;
-  static constexpr int kV = k8 ? 2 : (kPair ? 2 : 3);
+  static constexpr int kK = k8 ? 4 : 3;                      // (8 bits: K and V in turn)
+  static constexpr int kV = k8 ? 0 : (kPair ? 2 : 3);
   static constexpr int kRaw = k8 ? (kPair ? 2 : 3) : 0;
-  static constexpr uint32_t kSmem = (kQ + kK + kV) * kTileBytes + kRaw * (kRawBytes + 512) + 1024;
+  static constexpr int kRawScales = kRaw == 2 ? 1 : kRaw;    // (they come with K, which with two stages is always in the first)
+  // Powers of two of the scales: a K tile takes the place in the ring of the one two steps ago when its QK^T is complete; a softmax
+  // slot may then be a step behind that one, or with one query tile, whose slots have every other tile, two.
+  static constexpr int kPowers = kPair ? 4 : 8;
+  static constexpr uint32_t kSmem = (kQ + kK + kV) * kTileBytes + kRaw * kRawBytes + kRawScales * 1024 + 1024;
   static constexpr int kThreads = k8 ? 512 : 384;
   // setmaxnreg: what the roles ask for is what the block gets at launch
   static constexpr int kLaunchRegs = k8 ? 128 : 168;
@@ -45,7 +55,7 @@ template <int kFmt, bool kPair> struct Cfg {
   static constexpr int kSoftmax = k8 ? 192 : 208;
   static constexpr int kBlockRegs = 128 * kUtil + 256 * kSoftmax + (k8 ? 128 * kConvert : 0);
   static_assert(kBlockRegs <= kThreads * kLaunchRegs, "setmaxnreg would wait for ever");
-  static_assert(kSmem <= 231424 + 1024, "shared memory of an SM");
+  static_assert(kSmem <= 226 * 1024, "shared memory of an SM");
 };
 
 struct RowsParams {
@@ -65,10 +75,10 @@ struct RowsMaps {
 };
 
 struct Bars {
-  uint64_t q_full[2];
-  uint64_t k_full[3], k_empty[3];
+  uint64_t q_full[2], q_ready[2];
+  uint64_t k_full[4], k_empty[4];
   uint64_t v_full[3], v_empty[3];
-  uint64_t raw_full[3], raw_empty[3];
+  uint64_t raw_full[3], raw_empty[3], powers_full[8];
   uint64_t s_full[2], s_free, p_ready[2], pv_done[2];
 };
 
@@ -98,16 +108,6 @@ __device__ __forceinline__ void record_timeout(uint32_t* status, uint32_t site) 
   status[1] = site;
 }
 
-// Four codes times their scale, in q's type.
-template <bool kBF16, int kFmt>
-__device__ __forceinline__ void restore4(uint32_t w, float2 scale, uint32_t& lo, uint32_t& hi) {
-  uint32_t a, b;
-  codes_to_f16<kFmt>(w, a, b);
-  const float2 x = __fmul2_rn(unpack2<false>(a), scale), y = __fmul2_rn(unpack2<false>(b), scale);
-  lo = pack2<kBF16>(x.x, x.y);
-  hi = pack2<kBF16>(y.x, y.y);
-}
-
 // Grid: parts of the keys x blocks of query tiles x units, the blocks of a part side by side (they read the same keys).
 template <bool kBF16, int kFmt, bool kPair>
 __global__ void __launch_bounds__(Cfg<kFmt, kPair>::kThreads, 1)
@@ -115,13 +115,16 @@ attn_rows_kernel(const __grid_constant__ RowsMaps maps, const RowsParams p) {
   using C = Cfg<kFmt, kPair>;
   extern __shared__ uint8_t smem_raw[];
   __shared__ __align__(8) Bars bars;
+  // What the softmax needs of the scales of a tile's quarters: 2^e of the keys', e of the values' and 2^-e.
+  __shared__ float4 powers_s[C::k8 ? C::kPowers : 1][4];
+  __shared__ uint8_t unit_s[C::k8 && kBF16 ? C::kQ : 1][kTile];  // exponent of a query row's power of two, as f32 has it
   __shared__ float2 row_s[kPair ? 1 : kTile];  // (one tile) second slot's reference and sum; then both slots' factors
   __shared__ uint32_t tmem_base_s;
   __shared__ uint32_t abort_s;
 
   const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   const uint32_t sQ = smem_base, sK = sQ + C::kQ * kTileBytes, sV = sK + C::kK * kTileBytes;
-  const uint32_t sRaw = sV + C::kV * kTileBytes, sScale = sRaw + C::kRaw * kRawBytes;
+  const uint32_t sRaw = sV + C::kV * kTileBytes, sRawScale = sRaw + C::kRaw * kRawBytes;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   volatile uint32_t* abortp = &abort_s;
 
@@ -137,15 +140,19 @@ attn_rows_kernel(const __grid_constant__ RowsMaps maps, const RowsParams p) {
     abort_s = 0;
     for (int i = 0; i < 2; ++i) {
       mbar_init(smem_u32(&bars.q_full[i]), 1);
+      mbar_init(smem_u32(&bars.q_ready[i]), 128);
       mbar_init(smem_u32(&bars.s_full[i]), 1);
       mbar_init(smem_u32(&bars.p_ready[i]), 128);
       mbar_init(smem_u32(&bars.pv_done[i]), 1);
     }
     mbar_init(smem_u32(&bars.s_free), 128);
-    for (int i = 0; i < 3; ++i) {
-      mbar_init(smem_u32(&bars.k_full[i]), C::k8 ? 128 : 1);
+    for (int i = 0; i < 4; ++i) {
+      mbar_init(smem_u32(&bars.k_full[i]), C::k8 ? 4 : 1);
       mbar_init(smem_u32(&bars.k_empty[i]), 1);
-      mbar_init(smem_u32(&bars.v_full[i]), C::k8 ? 128 : 1);
+    }
+    for (int i = 0; i < C::kPowers; ++i) mbar_init(smem_u32(&bars.powers_full[i]), 4);
+    for (int i = 0; i < 3; ++i) {
+      mbar_init(smem_u32(&bars.v_full[i]), 1);
       mbar_init(smem_u32(&bars.v_empty[i]), 1);
       mbar_init(smem_u32(&bars.raw_full[i]), 1);
       mbar_init(smem_u32(&bars.raw_empty[i]), 4);
@@ -181,6 +188,25 @@ attn_rows_kernel(const __grid_constant__ RowsMaps maps, const RowsParams p) {
   const int n0 = kPair ? n : (n + 1) / 2;            // steps of either slot
   const int n1 = kPair ? (two ? n : 0) : n / 2;
 
+  // The stage of K or V tile c, its barriers and the use of it that this is.
+  struct Stage {
+    uint32_t at;
+    uint64_t *full, *empty;
+    int use;
+  };
+  auto k_stage = [&](int c) -> Stage {
+    const int u = C::k8 ? 2 * c : c, st = u % C::kK;
+    return {sK + st * kTileBytes, &bars.k_full[st], &bars.k_empty[st], u / C::kK};
+  };
+  auto v_stage = [&](int c) -> Stage {
+    if constexpr (C::k8) {
+      const int u = 2 * c + 1, st = u % C::kK;
+      return {sK + st * kTileBytes, &bars.k_full[st], &bars.k_empty[st], u / C::kK};
+    } else {
+      const int st = c % C::kV;
+      return {sV + st * kTileBytes, &bars.v_full[st], &bars.v_empty[st], c / C::kV};
+    }
+  };
   auto wait_all = [&](uint64_t* bar, uint32_t parity, uint32_t site) -> bool {
     const bool good = __all_sync(0xffffffffu, mbar_wait(smem_u32(bar), parity, abortp));
     if (!good && lane == 0) record_timeout(p.status, site);
@@ -213,9 +239,13 @@ attn_rows_kernel(const __grid_constant__ RowsMaps maps, const RowsParams p) {
           }
           if (use > 0) fence_proxy_async_smem();  // (the consumers' reads, behind the wait above, before the copy)
           const uint32_t bar = smem_u32(&bars.raw_full[st]);
-          mbar_expect_tx(bar, kRawBytes + 512);
+          mbar_expect_tx(bar, kRawBytes + (c & 1 ? 0u : 1024u));
           tma_load_4d(sRaw + st * kRawBytes, (c & 1) ? &maps.v : &maps.k, bar, 0, hk, key, seq);
-          tma_load_4d(sScale + st * 512, (c & 1) ? &maps.vs : &maps.ks, bar, key, hk, seq, 0);
+          if ((c & 1) == 0) {  // (both scales with the keys: the softmax needs them first)
+            const uint32_t at = sRawScale + st % C::kRawScales * 1024;
+            tma_load_4d(at, &maps.ks, bar, key, hk, seq, 0);
+            tma_load_4d(at + 512, &maps.vs, bar, key, hk, seq, 0);
+          }
         }
         if (!ok) {
           // give copies already in flight a bounded chance to land before the CTA retires
@@ -274,7 +304,7 @@ attn_rows_kernel(const __grid_constant__ RowsMaps maps, const RowsParams p) {
     // Step j of slot 0, step j of slot 1, step j + 1 of slot 0, ...: each when the softmax warps have the one before
     // it in registers.
     reg_dealloc<C::kUtil>();
-    constexpr uint32_t kFmtBits = kBF16 ? UMMA_BF16 : UMMA_F16;
+    constexpr uint32_t kFmtBits = kBF16 && !C::k8 ? UMMA_BF16 : UMMA_F16;
     constexpr uint32_t idesc = umma_idesc_f16(kFmtBits, UMMA_K_MAJOR, UMMA_K_MAJOR, 128, 128);
     bool ok = true;
     uint32_t uses = 0;  // of S so far
@@ -282,17 +312,17 @@ attn_rows_kernel(const __grid_constant__ RowsMaps maps, const RowsParams p) {
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
         if (j >= (t ? n1 : n0)) continue;
-        const int c = kPair ? j : 2 * j + t, st = c % C::kK;
-        const bool k_hit = mbar_try_wait(smem_u32(&bars.k_full[st]), (c / C::kK) & 1);
+        const Stage k = k_stage(kPair ? j : 2 * j + t);
+        const bool k_hit = mbar_try_wait(smem_u32(k.full), k.use & 1);
         const bool s_hit = uses == 0 || mbar_try_wait(smem_u32(&bars.s_free), (uses - 1) & 1);
-        if (j == 0 && (kPair || t == 0)) ok = wait_all(&bars.q_full[t], 0, 94);
-        if (ok && !__all_sync(0xffffffffu, k_hit)) ok = wait_all(&bars.k_full[st], (c / C::kK) & 1, 95);
+        if (j == 0 && (kPair || t == 0)) ok = wait_all(C::k8 && kBF16 ? &bars.q_ready[t] : &bars.q_full[t], 0, 94);
+        if (ok && !__all_sync(0xffffffffu, k_hit)) ok = wait_all(k.full, k.use & 1, 95);
         if (ok && !__all_sync(0xffffffffu, s_hit)) ok = wait_all(&bars.s_free, (uses - 1) & 1, 96);
         if (!ok) break;
         ++uses;
         tc_fence_after_sync();
         if (elect_one()) {
-          const uint64_t kdesc = umma_smem_desc_sw128(sK + st * kTileBytes, 16, 1024);
+          const uint64_t kdesc = umma_smem_desc_sw128(k.at, 16, 1024);
           const uint64_t qdesc = umma_smem_desc_sw128(sQ + (kPair ? t : 0) * kTileBytes, 16, 1024);
 #pragma unroll
           for (int kk = 0; kk < 8; ++kk) {
@@ -301,7 +331,7 @@ attn_rows_kernel(const __grid_constant__ RowsMaps maps, const RowsParams p) {
           }
           umma_commit(smem_u32(&bars.s_full[t]));
           // the K stage is free after the last QK^T that reads it
-          if (!kPair || t == 1 || !two) umma_commit(smem_u32(&bars.k_empty[st]));
+          if (!kPair || t == 1 || !two) umma_commit(smem_u32(k.empty));
         }
         __syncwarp();
       }
@@ -309,7 +339,7 @@ attn_rows_kernel(const __grid_constant__ RowsMaps maps, const RowsParams p) {
   } else if (warp == 3) {
     // ------------------------------------------------------------------ P.V issuer
     reg_dealloc<C::kUtil>();
-    constexpr uint32_t kFmtBits = kBF16 ? UMMA_BF16 : UMMA_F16;
+    constexpr uint32_t kFmtBits = kBF16 && !C::k8 ? UMMA_BF16 : UMMA_F16;
     constexpr uint32_t idesc = umma_idesc_f16(kFmtBits, UMMA_K_MAJOR, UMMA_MN_MAJOR, 128, 128);
     bool ok = true;
     int cleared = -1;
@@ -317,8 +347,9 @@ attn_rows_kernel(const __grid_constant__ RowsMaps maps, const RowsParams p) {
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
         if (j >= (t ? n1 : n0)) continue;
-        const int c = kPair ? j : 2 * j + t, st = c % C::kV;
-        ok = wait_all(&bars.v_full[st], (c / C::kV) & 1, 97);
+        const int c = kPair ? j : 2 * j + t;
+        const Stage v = v_stage(c);
+        ok = wait_all(v.full, v.use & 1, 97);
         if (!ok) break;
         if (!C::k8 && (j0 + c + 1) * kTile > len && cleared != c) {
           // what lies behind the sequence may be infinite or NaN, and its weights of 0 would not stop that
@@ -326,7 +357,7 @@ attn_rows_kernel(const __grid_constant__ RowsMaps maps, const RowsParams p) {
           const int live = len - (j0 + c) * kTile;
           const uint32_t zero[4] = {0, 0, 0, 0};
           for (int i = live * 16 + lane; i < kTile * 16; i += 32)
-            sts4(sV + st * kTileBytes + (i & 8) * (kHalfBytes / 8) + (i >> 4) * 128 + (i & 7) * 16, zero);
+            sts4(v.at + (i & 8) * (kHalfBytes / 8) + (i >> 4) * 128 + (i & 7) * 16, zero);
           fence_proxy_async_smem();
           __syncwarp();
         }
@@ -334,58 +365,126 @@ attn_rows_kernel(const __grid_constant__ RowsMaps maps, const RowsParams p) {
         if (!ok) break;
         tc_fence_after_sync();
         if (elect_one()) {
-          const uint64_t vdesc = umma_smem_desc_sw128(sV + st * kTileBytes, kHalfBytes, 1024);
+          const uint64_t vdesc = umma_smem_desc_sw128(v.at, kHalfBytes, 1024);
           const uint32_t tP = tbase + 128 + t * 64, tO = tbase + 256 + t * 128;
 #pragma unroll
           for (int kk = 0; kk < 8; ++kk)
             umma_ts(tO, tP + kk * 8, vdesc + static_cast<uint64_t>(kk * (2048 >> 4)), idesc, (j > 0 || kk > 0) ? 1u : 0u);
           umma_commit(smem_u32(&bars.pv_done[t]));
           // the V stage is free after the last P.V that reads it
-          if (!kPair || t == 1 || !two) umma_commit(smem_u32(&bars.v_empty[st]));
+          if (!kPair || t == 1 || !two) umma_commit(smem_u32(v.empty));
         }
         __syncwarp();
       }
     }
   } else if (warp >= 12) {
-    // ------------------------------------------------------------------ codes to 16-bit tiles, a row to a thread
+    // ------------------------------------------------------------------ codes to f16 tiles, a row to a thread
     if constexpr (C::k8) {
       reg_dealloc<C::kConvert>();
-      const int row = tid - 384;
       bool ok = true;
-      for (int c = 0; c < 2 * n; ++c) {
+      if constexpr (kBF16) {
+        const int row = tid - 384;
+        for (int t = 0; t < (two ? 2 : 1) && n > 0 && ok; ++t) {
+          ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&bars.q_full[t]), 0, abortp));
+          if (!ok) break;
+          float top = 0.f;
+#pragma unroll
+          for (int ch = 0; ch < 16; ++ch) {
+            uint32_t w[4];
+            lds4(sQ + t * kTileBytes + (ch >> 3) * kHalfBytes + sw128_offset(row, ch & 7), w);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const float2 v = unpack2<true>(w[i]);
+              top = max3(top, fabsf(v.x), fabsf(v.y));
+            }
+          }
+          // (rows of zeros, and of nothing but values under 2^-100, stay as they are or vanish)
+          const int e = min(max(static_cast<int>(__float_as_uint(top) >> 23), 27), 253);
+          const float down = __uint_as_float(static_cast<uint32_t>(254 - e) << 23);
+          unit_s[t][row] = static_cast<uint8_t>(e);
+#pragma unroll 4
+          for (int ch = 0; ch < 16; ++ch) {
+            const uint32_t at = sQ + t * kTileBytes + (ch >> 3) * kHalfBytes + sw128_offset(row, ch & 7);
+            uint32_t w[4];
+            lds4(at, w);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const float2 v = unpack2<true>(w[i]);
+              w[i] = pack2<false>(v.x * down, v.y * down);
+            }
+            sts4(at, w);
+          }
+          fence_proxy_async_smem();
+          mbar_arrive(smem_u32(&bars.q_ready[t]));
+        }
+      }
+      const int row = tid - 384;
+      float vs = 0.f;               // the row's value scale, from the keys' turn to the values'
+      float v_up = 0.f;             // 2^-e of the warp's 32
+      int v_least = -80;            // (e does not fall by more than 40 from its largest, nor so low that a row sum could suffer)
+      for (int c = 0; c < 2 * n && ok; ++c) {
         const int st = c % C::kRaw, j = c >> 1;
         const bool is_v = c & 1;
-        const int ring = is_v ? C::kV : C::kK, to = j % ring, use = j / ring;
+        const Stage to = is_v ? v_stage(j) : k_stage(j);
         ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&bars.raw_full[st]), (c / C::kRaw) & 1, abortp));
-        if (ok && use > 0)
-          ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(is_v ? &bars.v_empty[to] : &bars.k_empty[to]), (use - 1) & 1, abortp));
-        if (!ok) {
-          if (lane == 0) record_timeout(p.status, 99);
-          break;
-        }
-        const uint32_t src = sRaw + st * kRawBytes, dst = (is_v ? sV : sK) + to * kTileBytes;
+        if (!ok) break;
+        const uint32_t src = sRaw + st * kRawBytes;
         const bool live = (j0 + j) * kTile + row < len;  // (what lies behind the sequence may be anything)
-        const float f = ldsf(sScale + st * 512 + row * 4);
-        const float2 scale = make_float2(f, f);
+        uint32_t w[32];
+#pragma unroll
+        for (int ch = 0; ch < 8; ++ch) lds4(src + sw128_offset(row, ch), w + 4 * ch);
+        float scale;
+        if (!is_v) {
+          const uint32_t at = sRawScale + st % C::kRawScales * 1024 + row * 4;
+          scale = live ? ldsf(at) : 0.f;
+          vs = live ? ldsf(at + 512) : 0.f;
+          float k_top = fabsf(scale), v_top = fabsf(vs);
+#pragma unroll
+          for (int d = 16; d > 0; d >>= 1) {
+            k_top = fmaxf(k_top, __shfl_xor_sync(0xffffffffu, k_top, d));
+            v_top = fmaxf(v_top, __shfl_xor_sync(0xffffffffu, v_top, d));
+          }
+          const int ke = min(max(static_cast<int>(__float_as_uint(k_top) >> 23) - 127, -100), 126);
+          const int ve = min(max(static_cast<int>(__float_as_uint(v_top) >> 23) - 127, v_least), 126);
+          v_least = max(v_least, ve - 40);
+          v_up = __uint_as_float(static_cast<uint32_t>(127 - ve) << 23);
+          scale *= __uint_as_float(static_cast<uint32_t>(127 - ke) << 23);
+          if (lane == 0) {
+            powers_s[j % C::kPowers][warp - 12] = make_float4(__uint_as_float(static_cast<uint32_t>(127 + ke) << 23), static_cast<float>(ve), v_up, 0.f);
+            mbar_arrive(smem_u32(&bars.powers_full[j % C::kPowers]));
+          }
+        } else {
+          scale = vs * v_up;
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&bars.raw_empty[st]));
+        if (to.use > 0) {
+          ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(to.empty), (to.use - 1) & 1, abortp));
+          if (!ok) break;
+        }
+        const __half hi = __float2half_rn(scale), lo = __float2half_rn(scale - __half2float(hi));
+        const __half2 hi2 = __half2half2(hi), lo2 = __half2half2(lo);
 #pragma unroll
         for (int ch = 0; ch < 8; ++ch) {
-          uint32_t w[4], y[8];
-          lds4(src + sw128_offset(row, ch), w);
+          uint32_t y[8];
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            restore4<kBF16, kFmt>(w[i], scale, y[2 * i], y[2 * i + 1]);
-            y[2 * i] = live ? y[2 * i] : 0u;
-            y[2 * i + 1] = live ? y[2 * i + 1] : 0u;
+          for (int z = 0; z < 4; ++z) {
+            codes_to_f16<kFmt>(live ? w[4 * ch + z] : 0u, y[2 * z], y[2 * z + 1]);
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+              __half2& v = *reinterpret_cast<__half2*>(&y[2 * z + x]);
+              v = __hfma2(v, hi2, __hmul2(v, lo2));
+            }
           }
-          const uint32_t half = dst + (ch >> 2) * kHalfBytes;
+          const uint32_t half = to.at + (ch >> 2) * kHalfBytes;
           sts4(half + sw128_offset(row, (ch & 3) * 2), y);
           sts4(half + sw128_offset(row, (ch & 3) * 2 + 1), y + 4);
         }
         fence_proxy_async_smem();
-        mbar_arrive(smem_u32(is_v ? &bars.v_full[to] : &bars.k_full[to]));
         __syncwarp();
-        if (lane == 0) mbar_arrive(smem_u32(&bars.raw_empty[st]));
+        if (lane == 0) mbar_arrive(smem_u32(to.full));
       }
+      if (!ok && lane == 0) record_timeout(p.status, 99);
     }
   } else {
     // ------------------------------------------------------------------ softmax + epilogue
@@ -397,7 +496,7 @@ attn_rows_kernel(const __grid_constant__ RowsMaps maps, const RowsParams p) {
     const uint32_t tS = tbase + lane_base;
     const uint32_t tP = tbase + lane_base + 128 + t * 64;
     const uint32_t tO = tbase + lane_base + 256 + t * 128;
-    const float mul = p.scale_log2;
+    float mul = p.scale_log2;
     const int n_t = t ? n1 : n0;
     // this thread's query row
     const int tile = tile0 + (kPair ? t : 0);
@@ -427,31 +526,45 @@ attn_rows_kernel(const __grid_constant__ RowsMaps maps, const RowsParams p) {
       const int thr = lim - jk;  // columns > thr of this tile are masked for this row
       // The whole 128-wide row goes to registers at once, and S to the next QK^T.
       float e[128];
+      float4 power[4];  // (8 bits) of the tile's quarters
       {
         uint32_t(&u)[128] = *reinterpret_cast<uint32_t(*)[128]>(e);
         tmem_ld32(tS + 0, *reinterpret_cast<uint32_t(*)[32]>(&u[0]));
         tmem_ld32(tS + 32, *reinterpret_cast<uint32_t(*)[32]>(&u[32]));
         tmem_ld32(tS + 64, *reinterpret_cast<uint32_t(*)[32]>(&u[64]));
         tmem_ld32(tS + 96, *reinterpret_cast<uint32_t(*)[32]>(&u[96]));
+        if constexpr (C::k8) {
+          const int c = kPair ? j : 2 * j + t;  // the tile, of the CTA's
+          ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&bars.powers_full[c % C::kPowers]), (c / C::kPowers) & 1, abortp));
+#pragma unroll
+          for (int g = 0; g < 4; ++g) power[g] = powers_s[c % C::kPowers][g];
+        }
         tmem_wait_ld();
       }
+      if (C::k8 && !ok) { if (lane == 0) record_timeout(p.status, 103); break; }
       tc_fence_before_sync();
       mbar_arrive(smem_u32(&bars.s_free));
+      if (C::k8 && kBF16 && j == 0) mul = p.scale_log2 * __uint_as_float(static_cast<uint32_t>(unit_s[kPair ? t : 0][r_in_tile]) << 23);
       if (jk + kTile - 1 > min_lim) {
 #pragma unroll
         for (int i = 0; i < 128; ++i) e[i] = (i > thr) ? -INFINITY : e[i];
       }
       // The tile's row maximum is the reference of a first tile; a later one only moves the reference up
       // (and rescales what was accumulated under the old one) when it exceeds it by too much.
-      float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+      float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};  // of the quarters
 #pragma unroll
-      for (int i = 0; i < 128; i += 8) {
-        mx4[0] = max3(mx4[0], e[i], e[i + 1]);
-        mx4[1] = max3(mx4[1], e[i + 2], e[i + 3]);
-        mx4[2] = max3(mx4[2], e[i + 4], e[i + 5]);
-        mx4[3] = max3(mx4[3], e[i + 6], e[i + 7]);
+      for (int i = 0; i < 32; i += 2) {
+#pragma unroll
+        for (int g = 0; g < 4; ++g) mx4[g] = max3(mx4[g], e[32 * g + i], e[32 * g + i + 1]);
       }
-      const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * mul;
+      float mx;
+      if constexpr (C::k8) {
+        mx = -INFINITY;
+#pragma unroll
+        for (int g = 0; g < 4; ++g) mx = fmaxf(mx, fmaf(mx4[g], mul * power[g].x, power[g].y));
+      } else {
+        mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * mul;
+      }
       if (j == 0) {
         m_ref = mx;
       } else {
@@ -481,19 +594,36 @@ attn_rows_kernel(const __grid_constant__ RowsMaps maps, const RowsParams p) {
       }
       // two logits per FMA instruction (packed f32x2); P is packed to 16 bits right away
       const float ref = m_ref > -INFINITY ? m_ref : 0.f;
-      const float2 mul2 = make_float2(mul, mul), neg_m2 = make_float2(-ref, -ref);
       float2 ts4[4] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f), make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
       uint32_t pk[64];
+      if constexpr (C::k8) {
 #pragma unroll
-      for (int i = 0; i < 64; ++i) {
-        float2 v = __ffma2_rn(make_float2(e[2 * i], e[2 * i + 1]), mul2, neg_m2);
-        v.x = ex2(v.x);
-        v.y = ex2(v.y);
-        ts4[i & 3] = __fadd2_rn(ts4[i & 3], v);
-        pk[i] = pack2<kBF16>(v.x, v.y);
+        for (int g = 0; g < 4; ++g) {
+          const float f = mul * power[g].x, up = power[g].y - ref;
+          const float2 mul2 = make_float2(f, f), up2 = make_float2(up, up);
+#pragma unroll
+          for (int i = 16 * g; i < 16 * g + 16; ++i) {
+            float2 v = __ffma2_rn(make_float2(e[2 * i], e[2 * i + 1]), mul2, up2);
+            v.x = ex2(v.x);
+            v.y = ex2(v.y);
+            ts4[g] = __fadd2_rn(ts4[g], v);
+            pk[i] = pack2<false>(v.x, v.y);
+          }
+          l = fmaf(ts4[g].x + ts4[g].y, power[g].z, l);
+        }
+      } else {
+        const float2 mul2 = make_float2(mul, mul), neg_m2 = make_float2(-ref, -ref);
+#pragma unroll
+        for (int i = 0; i < 64; ++i) {
+          float2 v = __ffma2_rn(make_float2(e[2 * i], e[2 * i + 1]), mul2, neg_m2);
+          v.x = ex2(v.x);
+          v.y = ex2(v.y);
+          ts4[i & 3] = __fadd2_rn(ts4[i & 3], v);
+          pk[i] = pack2<kBF16>(v.x, v.y);
+        }
+        const float2 ts2 = __fadd2_rn(__fadd2_rn(ts4[0], ts4[1]), __fadd2_rn(ts4[2], ts4[3]));
+        l += ts2.x + ts2.y;
       }
-      const float2 ts2 = __fadd2_rn(__fadd2_rn(ts4[0], ts4[1]), __fadd2_rn(ts4[2], ts4[3]));
-      l += ts2.x + ts2.y;
       if (j > 0) {  // P_t is free when the last P.V has read it
         ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&bars.pv_done[t]), (j - 1) & 1, abortp));
         if (!ok) { if (lane == 0) record_timeout(p.status, 101); break; }
@@ -734,7 +864,8 @@ cudaError_t launch_rows_of(const CacheRows& c, const CacheAttnArgs& a, RowsParam
   RowsMaps maps;
   const uint32_t box[4] = {64, static_cast<uint32_t>(p.q.group), static_cast<uint32_t>(tiles.pos), static_cast<uint32_t>(tiles.b)};
   if (tma_host::make_boxed_map(&maps.q, a.q, kBF16, a.B, a.Sq, a.H, 128, a.q_sb, a.q_ss, a.q_sh, box) ||
-      make_rows_map(&maps.k, c, false, p.q.Hkv, kBF16, kTile) || make_rows_map(&maps.v, c, true, p.q.Hkv, kBF16, kTile))
+      make_rows_map(&maps.k, c, false, p.q.Hkv, kBF16, kTile) ||
+      make_rows_map(&maps.v, c, true, p.q.Hkv, kBF16, kTile))
     return cudaErrorInvalidValue;
   if (C::k8) {
     if (make_scale_map(&maps.ks, c, false, p.q.Hkv, kTile) || make_scale_map(&maps.vs, c, true, p.q.Hkv, kTile))

@@ -6,8 +6,9 @@ its roundings add up to, which `_attention` bounds for every output from the sam
   - the output's own rounding, `half` = finfo(q.dtype).eps / 2 of it;
   - the weights' before the second product: `half` of each (f16, 2^-11, or bf16, 2^-8), and 2^-25 of the largest
     where a weight is subnormal in f16;
-  - where rows of more than one tile read an 8-bit cache, its values' rounding to q's type: `half` of each key's (a logit
-    then moves by half * sum |q k|) and of each value's;
+  - over an 8-bit cache, bf16 queries as f16 under a power of two: 2^-25 of a row's largest value in every term; and keys and values,
+    where more than 16 rows use them, as f16 under a power of two of the largest of 32: 2^-11 of each, 2^-24 of the
+    largest where it is subnormal;
   - f32 arithmetic: 2^-24 for each of a dot product's 128 terms, 2^-20 for an exponential, 2^-22 for each of the few rescalings.
 """
 import ctypes
@@ -104,7 +105,6 @@ def _attention(q, cache, kv_len=None, causal=True, prefix=None, prefix_len=None,
   Hkv = cache.k.shape[2]
   group = H // Hkv
   half = torch.finfo(q.dtype).eps / 2
-  eight = cache.k_scale is not None or (prefix is not None and prefix.k_scale is not None)
   out, lse = torch.zeros(q.shape, dtype=torch.float64, device="cuda"), torch.empty(B, H, Sq, dtype=torch.float64, device="cuda")
   tol, lse_tol = torch.empty_like(out), torch.empty_like(lse)
   for b in range(B):
@@ -132,9 +132,14 @@ def _attention(q, cache, kv_len=None, causal=True, prefix=None, prefix_len=None,
     o = torch.where(l > 0, p @ v / l.clamp(min=1e-300), 0.0)
     a = torch.where(l > 0, p @ v.abs() / l.clamp(min=1e-300), 0.0)
     most = v.abs().amax() if v.numel() else 0.0
-    by_logit = (128 * 2.0 ** -24 + (half if eight else 0)) * absdot + 2.0 ** -20
+    # (2^-25 of a query row's largest value against the largest key, 2^-24 of the largest key value against the query)
+    eight = cache.k_scale is not None or (prefix is not None and prefix.k_scale is not None)
+    small = (2.0 ** -25 * qs.abs().amax(-1) * (k.abs().sum(-1).amax() if k.numel() else 0.0) +
+             2.0 ** -24 * qs.abs().sum(-1) * (k.abs().amax() if k.numel() else 0.0)) * scale if eight else 0.0
+    by_logit = (128 * 2.0 ** -24 + (2.0 ** -11 if eight else 0)) * absdot + small + 2.0 ** -20
     of_weight = torch.expm1(2 * by_logit)[..., None] + half + 2.0 ** -18
-    bound = half * o.abs() + of_weight * (a + o.abs()) * 1.02 + (half * a if eight else 0) + s.shape[-1] * 2.0 ** -25 * most
+    of_value = 2.0 ** -11 * a + 2.0 ** -24 * most if eight else 0.0
+    bound = half * o.abs() + of_weight * (a + o.abs()) * 1.02 + of_value + s.shape[-1] * 2.0 ** -25 * most
     put = lambda t: t.permute(2, 0, 1, 3).reshape(Sq, H, D)
     out[b], tol[b] = put(o), put(bound)
     lse[b] = (top[..., 0] / 0.6931471805599453 + torch.log2(l[..., 0])).reshape(H, Sq)
