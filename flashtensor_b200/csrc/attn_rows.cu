@@ -438,14 +438,14 @@ attn_rows_kernel(const __grid_constant__ RowsMaps maps, const RowsParams p) {
           const uint32_t at = sRawScale + st % C::kRawScales * 1024 + row * 4;
           scale = live ? ldsf(at) : 0.f;
           vs = live ? ldsf(at + 512) : 0.f;
-          float k_top = fabsf(scale), v_top = fabsf(vs);
-#pragma unroll
-          for (int d = 16; d > 0; d >>= 1) {
-            k_top = fmaxf(k_top, __shfl_xor_sync(0xffffffffu, k_top, d));
-            v_top = fmaxf(v_top, __shfl_xor_sync(0xffffffffu, v_top, d));
-          }
-          const int ke = min(max(static_cast<int>(__float_as_uint(k_top) >> 23) - 127, -100), 126);
-          const int ve = min(max(static_cast<int>(__float_as_uint(v_top) >> 23) - 127, v_least), 126);
+          // exponents of the largest of the warp's 32 keys (of what is finite: the others are what they are)
+          auto bits = [](float x) {
+            const uint32_t b = __float_as_uint(x) & 0x7fffffffu;
+            return b < 0x7f800000u ? b : 0u;
+          };
+          const int k_top = static_cast<int>(__reduce_max_sync(0xffffffffu, bits(scale)) >> 23) - 127;
+          const int v_top = static_cast<int>(__reduce_max_sync(0xffffffffu, bits(vs)) >> 23) - 127;
+          const int ke = min(max(k_top, -100), 126), ve = min(max(v_top, v_least), 126);
           v_least = max(v_least, ve - 40);
           v_up = __uint_as_float(static_cast<uint32_t>(127 - ve) << 23);
           scale *= __uint_as_float(static_cast<uint32_t>(127 - ke) << 23);
@@ -455,6 +455,10 @@ attn_rows_kernel(const __grid_constant__ RowsMaps maps, const RowsParams p) {
           }
         } else {
           scale = vs * v_up;
+        }
+        if (!live) {  // (codes may be NaN)
+#pragma unroll
+          for (int i = 0; i < 32; ++i) w[i] = 0u;
         }
         __syncwarp();
         if (lane == 0) mbar_arrive(smem_u32(&bars.raw_empty[st]));
@@ -469,7 +473,7 @@ attn_rows_kernel(const __grid_constant__ RowsMaps maps, const RowsParams p) {
           uint32_t y[8];
 #pragma unroll
           for (int z = 0; z < 4; ++z) {
-            codes_to_f16<kFmt>(live ? w[4 * ch + z] : 0u, y[2 * z], y[2 * z + 1]);
+            codes_to_f16<kFmt>(w[4 * ch + z], y[2 * z], y[2 * z + 1]);
 #pragma unroll
             for (int x = 0; x < 2; ++x) {
               __half2& v = *reinterpret_cast<__half2*>(&y[2 * z + x]);
