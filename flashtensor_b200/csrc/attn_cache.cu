@@ -42,12 +42,14 @@ template <int kFmt> struct Tile {
   static constexpr int kKeys = kFmt == CACHE_16 ? 16 : 32;
   static constexpr uint32_t kHalf = 2048;                  // (16 bits) one 64-column half of the keys or values
   static constexpr uint32_t kK = 4096;                     // the keys, and the values
-  static constexpr uint32_t kScales = kFmt == CACHE_16 ? 0 : 2 * kKeys * 4;
 };
 constexpr uint32_t kTileBytes = 8192;
 
 struct StreamParams {
   Segment s[2];    // numbered through in this order
+  const float* k_scale[2];
+  const float* v_scale[2];
+  int64_t ks_sb[2], ks_sh[2], vs_sb[2], vs_sh[2];
   int segments;
   RowShape q;
   float scale_log2;
@@ -63,7 +65,7 @@ struct StreamParams {
 };
 struct StreamMaps {
   struct {
-    CUtensorMap k, v, ks, vs;
+    CUtensorMap k, v;
   } s[2];
 };
 
@@ -78,10 +80,11 @@ __device__ __forceinline__ void ldsm4_t(uint32_t addr, uint32_t (&r)[4]) {
 __device__ __forceinline__ void lds4(uint32_t addr, uint32_t* r) {
   asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
 }
-__device__ __forceinline__ float ldsf(uint32_t addr) {
-  float v;
-  asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
-  return v;
+__device__ __forceinline__ void prefetch_l2(const void* p) { asm volatile("prefetch.global.L2 [%0];" ::"l"(p)); }
+// x / y, y > 0, in 32 bits where they fit (a 64-bit division takes 0.2 us)
+__device__ __forceinline__ int64_t quotient(int64_t x, int64_t y) {
+  if (static_cast<uint64_t>(x | y) >> 32 == 0) return static_cast<uint32_t>(x) / static_cast<uint32_t>(y);
+  return x / y;
 }
 // an 8x8 block of 16-bit values, rows and columns exchanged
 __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
@@ -116,8 +119,6 @@ attn_stream_kernel(const __grid_constant__ StreamMaps maps, const StreamParams p
   extern __shared__ uint8_t smem_raw[];
   __shared__ __align__(8) uint64_t full[kWarps][kStages];
   __shared__ uint32_t abort_s;
-  __shared__ int64_t ahead_s[kThreads];  // tiles ahead of a thread's sequences
-  __shared__ int64_t warp_sum_s[kWarps];
 
   const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -138,7 +139,9 @@ attn_stream_kernel(const __grid_constant__ StreamMaps maps, const StreamParams p
   if (!p.chained) griddep_wait();
   griddep_launch_dependents();
 
-  // ---- the deal: every CTA adds up the tiles of all sequences (a thread has `per` consecutive ones)
+  __syncthreads();
+
+  // ---- the deal: every warp adds up the tiles of all sequences by itself (a lane has `per` consecutive ones)
   const int n_seqs = p.s[0].N + (p.segments > 1 ? p.s[1].N : 0);
   auto at = [&](int i, Cursor& c) {  // sequence i of all segments
     c.seg = i >= p.s[0].N ? 1 : 0;
@@ -146,31 +149,23 @@ attn_stream_kernel(const __grid_constant__ StreamMaps maps, const StreamParams p
     c.len = seen_of(p.s[c.seg], c.seq);
     c.tiles = (c.len + T::kKeys - 1) / T::kKeys;
   };
-  const int per = (n_seqs + kThreads - 1) / kThreads;
-  int64_t mine = 0;
-  for (int i = tid * per; i < min(n_seqs, (tid + 1) * per); ++i) {
+  const int per = (n_seqs + 31) / 32;
+  int64_t upto = 0;
+#pragma unroll 4
+  for (int i = lane * per; i < min(n_seqs, (lane + 1) * per); ++i) {
     Cursor c;
     at(i, c);
-    mine += static_cast<int64_t>(c.tiles) * p.q.Hkv;
+    upto += c.tiles;
   }
-  int64_t upto = mine;
 #pragma unroll
   for (int d = 1; d < 32; d <<= 1) {
     const int64_t x = __shfl_up_sync(0xffffffffu, upto, d);
     if (lane >= d) upto += x;
   }
-  if (lane == 31) warp_sum_s[warp] = upto;
-  __syncthreads();
-  int64_t before = 0, total = 0;
-#pragma unroll
-  for (int x = 0; x < kWarps; ++x) {
-    if (x < warp) before += warp_sum_s[x];
-    total += warp_sum_s[x];
-  }
-  ahead_s[tid] = before + upto - mine;
+  upto *= p.q.Hkv;  // tiles of this lane's sequences and those before
+  const int64_t total = __shfl_sync(0xffffffffu, upto, 31);
   const int64_t workers = static_cast<int64_t>(gridDim.x) * kWarps;
-  const int64_t share = max((total + workers - 1) / workers, static_cast<int64_t>(kMinTiles));
-  __syncthreads();
+  const int64_t share = max(static_cast<int64_t>(quotient(total + workers - 1, workers)), static_cast<int64_t>(kMinTiles));
 
   // (neighbours in the numbering on different SMs, so that a small launch uses all of them)
   const int64_t worker = static_cast<int64_t>(warp) * gridDim.x + blockIdx.x;
@@ -183,20 +178,18 @@ attn_stream_kernel(const __grid_constant__ StreamMaps maps, const StreamParams p
 
   Cursor c;
   {
-    int x = 0;  // the last thread whose sequences begin at or before the range
-    for (int step = 256; step > 0; step >>= 1)
-      if (x + step < kThreads && ahead_s[x + step] <= lo) x += step;
-    int i = x * per;
-    int64_t rest = lo - ahead_s[x];
-    for (;; ++i) {  // (bounded, should another stream change the lengths in between)
+    const int x = __ffs(__ballot_sync(0xffffffffu, upto > lo)) - 1;  // the lane whose sequences the range begins in
+    int64_t rest = lo - (x > 0 ? __shfl_sync(0xffffffffu, upto, max(x - 1, 0)) : 0);
+    for (int i = x * per;; ++i) {  // (bounded, should another stream change the lengths in between)
       at(i, c);
       const int64_t in_seq = static_cast<int64_t>(c.tiles) * p.q.Hkv;
       if (rest < in_seq || i + 1 == n_seqs) break;
       rest -= in_seq;
     }
     c.tiles = max(c.tiles, 1);
-    c.hk = static_cast<int>(min(rest / c.tiles, static_cast<int64_t>(p.q.Hkv - 1)));
-    c.tile = static_cast<int>(rest % c.tiles);
+    const int64_t hk = quotient(rest, c.tiles);
+    c.hk = static_cast<int>(min(hk, static_cast<int64_t>(p.q.Hkv - 1)));
+    c.tile = static_cast<int>(min(rest - hk * c.tiles, static_cast<int64_t>(c.tiles - 1)));
   }
   auto advance = [&](Cursor& x) {  // (only where a tile follows)
     if (++x.tile < x.tiles) return;
@@ -210,18 +203,25 @@ attn_stream_kernel(const __grid_constant__ StreamMaps maps, const StreamParams p
     }
   };
 
+  // The query rows of a unit whose keys are next, to L2: behind the first tiles, of which all warps ask for at once, they would
+  // wait for 4 us.
+  auto prefetch_rows = [&](const Cursor& x) {
+    const Segment& s = p.s[x.seg];
+#pragma unroll
+    for (int y = 0; y < kOct; ++y) {
+      const Row row = decode_row(min(8 * y + (lane >> 2), s.rows - 1), x.seq, x.hk, s, p.q);
+      prefetch_l2(p.qp + row.b * p.q_sb + row.pos * p.q_ss + row.h * p.q_sh + (lane & 3) * 32);
+    }
+  };
   const uint32_t ring = smem_base + warp * kStages * kTileBytes;
-  const uint32_t scales = smem_base + kWarps * kStages * kTileBytes + warp * kStages * T::kScales;
   auto fetch = [&](const Cursor& x, int st) {
     const uint32_t bar = smem_u32(&full[warp][st]), dst = ring + st * kTileBytes;
     const auto& m = maps.s[x.seg];
     const int key = x.tile * T::kKeys;
-    mbar_expect_tx(bar, kTileBytes + T::kScales);
+    mbar_expect_tx(bar, kTileBytes);
     tma_load_4d(dst, &m.k, bar, 0, x.hk, key, x.seq);
     if constexpr (k8) {
       tma_load_4d(dst + T::kK, &m.v, bar, 0, x.hk, key, x.seq);
-      tma_load_4d(scales + st * T::kScales, &m.ks, bar, key, x.hk, x.seq, 0);
-      tma_load_4d(scales + st * T::kScales + T::kKeys * 4, &m.vs, bar, key, x.hk, x.seq, 0);
     } else {
       tma_load_4d(dst + T::kHalf, &m.k, bar, 64, x.hk, key, x.seq);
       tma_load_4d(dst + T::kK, &m.v, bar, 0, x.hk, key, x.seq);
@@ -229,11 +229,27 @@ attn_stream_kernel(const __grid_constant__ StreamMaps maps, const StreamParams p
     }
   };
 
+  // Key lane's scales of the fetched tiles (8 bits), in the order of the tiles.
+  float ks_of[kStages], vs_of[kStages];
+  auto fetch_scales = [&](const Cursor& x, float& ks, float& vs) {
+    if constexpr (k8) {
+      const int key = x.tile * T::kKeys + lane;
+      const bool live = key < x.len;  // (what lies behind the sequence may be anything)
+      ks = live ? __ldcg(p.k_scale[x.seg] + x.seq * p.ks_sb[x.seg] + x.hk * p.ks_sh[x.seg] + key) : 0.f;
+      vs = live ? __ldcg(p.v_scale[x.seg] + x.seq * p.vs_sb[x.seg] + x.hk * p.vs_sh[x.seg] + key) : 0.f;
+    }
+  };
+
   Cursor ahead = c;  // the next tile to fetch
   int fetched = 0;
-  for (; fetched < kStages && fetched < count; ++fetched) {
-    if (lane == 0) fetch(ahead, fetched);
-    if (fetched + 1 < count) advance(ahead);
+  prefetch_rows(c);
+#pragma unroll
+  for (int i = 0; i < kStages; ++i) {
+    if (i >= count) continue;
+    if (lane == 0) fetch(ahead, i);
+    fetch_scales(ahead, ks_of[i], vs_of[i]);
+    ++fetched;
+    if (fetched < count) advance(ahead);
   }
 
   const int r0 = lane >> 2, t4 = lane & 3;
@@ -304,7 +320,7 @@ attn_stream_kernel(const __grid_constant__ StreamMaps maps, const StreamParams p
       if (first == 0 && lane == 0) {
         const int rest = c.tiles - (count - n);  // behind this worker's range
         p.deal[c.seg].workers[static_cast<int64_t>(c.seq) * p.q.Hkv + c.hk] =
-            make_int2(static_cast<int>(worker), static_cast<int>(worker + (rest > 0 ? (rest + share - 1) / share : 0)));
+            make_int2(static_cast<int>(worker), static_cast<int>(worker + (rest > 0 ? quotient(rest + share - 1, share) : 0)));
       }
     }
 
@@ -317,7 +333,7 @@ attn_stream_kernel(const __grid_constant__ StreamMaps maps, const StreamParams p
       }
       break;
     }
-    const uint32_t sK = ring + st * kTileBytes, sV = sK + T::kK, sKs = scales + st * T::kScales, sVs = sKs + T::kKeys * 4;
+    const uint32_t sK = ring + st * kTileBytes, sV = sK + T::kK;
     const int key0 = c.tile * T::kKeys;
     // s[u][y][e]: key 16 u + r0 (e < 2) or 16 u + 8 + r0, query row 8 y + 2 t4 + (e & 1)
     float s[kSub][kOct][4];
@@ -345,8 +361,8 @@ attn_stream_kernel(const __grid_constant__ StreamMaps maps, const StreamParams p
       }
 #pragma unroll
       for (int j = 0; j < 2 * kSub; ++j) {
-        ks[j] = ldsf(sKs + (8 * j + r0) * 4);
-        vs[j] = ldsf(sVs + (8 * j + r0) * 4);
+        ks[j] = __shfl_sync(0xffffffffu, ks_of[0], 8 * j + r0);
+        vs[j] = __shfl_sync(0xffffffffu, vs_of[0], 8 * j + r0);
       }
     } else {
       // this lane's row of the 8x8 blocks: keys 0-7 and 8-15, columns 0-7 and 8-15
@@ -384,7 +400,6 @@ attn_stream_kernel(const __grid_constant__ StreamMaps maps, const StreamParams p
 #pragma unroll
             for (int x = 0; x < 2; ++x)
               if (key > lim[y][x]) s[u][y][2 * z + x] = -INFINITY;
-          if (k8 && key >= c.len) vs[2 * u + z] = 0.f;
         }
     }
     float w[kOct][2];
@@ -487,11 +502,18 @@ attn_stream_kernel(const __grid_constant__ StreamMaps maps, const StreamParams p
       }
     }
     __syncwarp();
+#pragma unroll
+    for (int i = 0; i + 1 < kStages; ++i) {
+      ks_of[i] = ks_of[i + 1];
+      vs_of[i] = vs_of[i + 1];
+    }
     if (fetched < count) {
       if (lane == 0) {
         fence_proxy_async_smem();  // (the warp's reads of the stage before the copy)
         fetch(ahead, st);
       }
+      fetch_scales(ahead, ks_of[kStages - 1], vs_of[kStages - 1]);
+      if (ahead.tile == 0) prefetch_rows(ahead);
       ++fetched;
       if (fetched < count) advance(ahead);
     }
@@ -577,14 +599,14 @@ cudaError_t launch_stream_fmt(const CacheRows* const* c, StreamParams& p, bool b
     const CacheRows& r = *c[x < p.segments ? x : 0];
     if (make_rows_map(&m.k, r, false, p.q.Hkv, bf16, T::kKeys) || make_rows_map(&m.v, r, true, p.q.Hkv, bf16, T::kKeys))
       return cudaErrorInvalidValue;
-    if (kFmt != CACHE_16) {
-      if (make_scale_map(&m.ks, r, false, p.q.Hkv, T::kKeys) || make_scale_map(&m.vs, r, true, p.q.Hkv, T::kKeys))
-        return cudaErrorInvalidValue;
-    } else {
-      m.ks = m.vs = m.k;
-    }
+    p.k_scale[x] = r.k_scale;
+    p.v_scale[x] = r.v_scale;
+    p.ks_sb[x] = r.ks_sb;
+    p.ks_sh[x] = r.ks_sh;
+    p.vs_sb[x] = r.vs_sb;
+    p.vs_sh[x] = r.vs_sh;
   }
-  const uint32_t smem = kWarps * kStages * (kTileBytes + T::kScales) + 1024;
+  const uint32_t smem = kWarps * kStages * kTileBytes + 1024;
   bool wide = false;
   for (int x = 0; x < p.segments; ++x) wide = wide || p.s[x].rows > 8;
   const auto kern = bf16 ? (wide ? attn_stream_kernel<true, kFmt, 2> : attn_stream_kernel<true, kFmt, 1>)
