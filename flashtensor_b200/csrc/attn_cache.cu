@@ -5,7 +5,7 @@
 // heads of the group at all new positions, and for a prefix those of all sequences that share it.  A segment leaves, for every
 // query row, an unnormalised output, the reference of its exponentials and their sum; the last one merges and divides.
 //
-// attn_stream_kernel, for up to 16 rows to a unit: the keys and values are used by so few rows that the work is one read of the
+// attn_stream_kernel, for up to 16 rows to a unit (see `streams`): the keys and values are used by so few rows that the work is one read of the
 // cache, and the floor its bytes over the HBM bandwidth.  Sequences are of any lengths, known on the device only, and units may be
 // many and short or few and long; so the work is dealt out there:
 //   - a unit's keys are tiles of 32 (8 bits) or 16 (16 bits), 8 KB of keys and values, and the tiles of all units of all segments are
@@ -626,8 +626,19 @@ cudaError_t launch_stream(const CacheRows* const* c, StreamParams& p, bool bf16,
   }
 }
 
-// Query rows are few enough for the stream's one 16-row tile.
-bool streams(const Segment& s) { return s.rows <= kRows; }
+// Which kernel takes a segment of up to 16 rows to a unit; the other one's tiles (attn_rows.cu) are mostly empty then, but
+// 16-bit keys come in copies four times as large and need no instruction of a warp.  It has a CTA for a unit, or several,
+// and nothing to follow a short one; the stream is even whatever the units are.  Streamed / tiles, us:
+//   16 bits, 4 rows   8 units 1024 keys 8.7/7.7, 8000 keys 17.7/14.6; 32 units 4001 keys 18.1/16.6, 128 units 43.8/41.4;
+//                     128 units 16384 keys 140/135; 256 units 1000 keys 26.6/28.4, 512 units 500 keys 26.7/39.4
+//   16 bits, 16 rows  16 units 8003 keys 25.3/17.2, 128 units 4001 keys 52/43
+//   8 bits, 4 rows    8 units 1024 keys 8.4/8.6, 8000 keys 13.7/15.0; 128 units 4001 keys 30.6/57.8
+//   8 bits, 16 rows   16 units 8003 keys 26/20; 8 units 32000 keys 34/37; 128 units 4001 keys 44/58
+bool streams(const Segment& s, const RowShape& q, int format, int num_sms) {
+  if (s.rows > kRows) return false;
+  const int64_t units = static_cast<int64_t>(s.N) * q.Hkv;
+  return format == CACHE_16 ? units > num_sms : s.rows <= 8 || 4 * units > num_sms;
+}
 
 size_t row_count(const CacheAttnArgs& a) { return static_cast<size_t>(a.B) * a.Sq * a.H; }
 
@@ -649,6 +660,7 @@ struct Plan {
   Segment s[2];        // prefix, own
   const CacheRows* c[2];
   bool have[2], stream[2], together;
+  bool finished;       // the own rows' kernel leaves nothing to merge
   Source from[2];      // partial results
   size_t bytes;
 };
@@ -664,8 +676,9 @@ Plan plan_of(const CacheAttnArgs& a, void* ws, int num_sms) {
     x.from[i] = Source{};
     if (!x.have[i]) continue;
     x.s[i] = segment_of(*x.c[i], a, i == 1 && a.causal);
-    x.stream[i] = streams(x.s[i]);
+    x.stream[i] = streams(x.s[i], q, x.c[i]->format, num_sms);
   }
+  x.finished = false;
   x.together = x.stream[0] && x.stream[1] && a.prefix.format == a.own.format;
   Carver w{static_cast<uint8_t*>(ws), 0};
   const size_t rows = row_count(a), workers = static_cast<size_t>(num_sms) * kWarps;
@@ -676,6 +689,8 @@ Plan plan_of(const CacheAttnArgs& a, void* ws, int num_sms) {
     f.dealt = x.stream[i];
     if (!f.dealt) {
       f.fixed.parts = attn_rows_parts(x.s[i], q, num_sms);
+      x.finished = !x.have[0] && f.fixed.parts == 1;
+      if (x.finished) continue;
       f.fixed.o = w.take<float>(rows * f.fixed.parts * 128);
       f.fixed.ml = w.take<float>(rows * f.fixed.parts * 2);
       continue;
@@ -720,20 +735,22 @@ cudaError_t launch_attn_cache(const CacheAttnArgs& a, void* ws, int num_sms, cud
   p.status = device_status_words();
   for (int i = 0; i < 2; ++i) {
     if (!x.have[i] || (i == 1 && x.together)) continue;
+    const bool chained = i == 1 && x.have[0];
     cudaError_t e;
     if (x.stream[i]) {
       p.segments = x.together ? 2 : 1;
-      p.chained = i == 1 && x.have[0] ? 1 : 0;
+      p.chained = chained ? 1 : 0;
       for (int y = 0; y < p.segments; ++y) {
         p.s[y] = x.s[i + y];
         p.deal[y] = x.from[i + y].deal;
       }
       e = launch_stream(x.c + i, p, a.bf16, num_sms, stream);
     } else {
-      e = launch_attn_rows(*x.c[i], x.s[i], a, x.from[i].fixed, stream);
+      e = launch_attn_rows(*x.c[i], x.s[i], a, x.from[i].fixed, x.finished, chained, stream);
     }
     if (e != cudaSuccess) return e;
   }
+  if (x.finished) return cudaSuccess;
   return launch_attn_merge(a, x.from[0], x.from[1], p.finish != 0 && x.stream[1], num_sms * kWarps, stream);
 }
 

@@ -128,9 +128,11 @@ inline int make_scale_map(CUtensorMap* m, const CacheRows& c, bool values, int H
   return tma_host::make_f32_map(m, values ? c.v_scale : c.k_scale, dims, strides, boxes, false);
 }
 
-// attn_rows.cu: a segment of more than 16 rows to a unit leaves its partial results at `mine` (mine.parts of each row)
+// attn_rows.cu: a segment leaves its partial results at `mine` (mine.parts of each row), or with `finish`, one part that is all there
+// is, the output
 int attn_rows_parts(const Segment& s, const RowShape& q, int num_sms);
-cudaError_t launch_attn_rows(const CacheRows& c, const Segment& s, const CacheAttnArgs& a, const Partials& mine, cudaStream_t stream);
+cudaError_t launch_attn_rows(const CacheRows& c, const Segment& s, const CacheAttnArgs& a, const Partials& mine, bool finish,
+                             bool chained, cudaStream_t stream);
 // ... and the output is what the partial results of up to two segments add up to.  `finished`: units that lay in one range are the
 // output already.
 cudaError_t launch_attn_merge(const CacheAttnArgs& a, const Source& first, const Source& second, bool finished, int workers,

@@ -67,6 +67,10 @@ struct RowsParams {
   int parts;
   float scale_log2;
   Partials mine;
+  uint16_t* out;          // (kFinish)
+  int64_t o_sb, o_ss, o_sh;
+  float* lse2;
+  int chained;            // as the stream's (attn_cache.cu)
   uint32_t* status;
 };
 
@@ -109,7 +113,9 @@ __device__ __forceinline__ void record_timeout(uint32_t* status, uint32_t site) 
 }
 
 // Grid: parts of the keys x blocks of query tiles x units, the blocks of a part side by side (they read the same keys).
-template <bool kBF16, int kFmt, bool kPair>
+// kFinish: one part that is all there is, and the output instead of partial results (an instantiation of its own: what a CTA does
+// once it also fetches its instructions for, and both ways in one kernel took 1.2 us longer).
+template <bool kBF16, int kFmt, bool kPair, bool kFinish>
 __global__ void __launch_bounds__(Cfg<kFmt, kPair>::kThreads, 1)
 attn_rows_kernel(const __grid_constant__ RowsMaps maps, const RowsParams p) {
   using C = Cfg<kFmt, kPair>;
@@ -171,7 +177,7 @@ attn_rows_kernel(const __grid_constant__ RowsMaps maps, const RowsParams p) {
   __syncthreads();
   tc_fence_after_sync();
   const uint32_t tbase = tmem_base_s;
-  griddep_wait();
+  if (!p.chained) griddep_wait();
   griddep_launch_dependents();
 
   // This CTA's key tiles: its part of what the sequence has, and of what the block's last rows see.
@@ -505,7 +511,7 @@ attn_rows_kernel(const __grid_constant__ RowsMaps maps, const RowsParams p) {
     // this thread's query row
     const int tile = tile0 + (kPair ? t : 0);
     bool live = (!kPair || t == 0 || two) && r_in_tile < p.tile_b * p.tile_pos * p.q.group;
-    int64_t number = 0;
+    int64_t number = 0, out_at = 0, lse_at = 0;
     int lim = len - 1, min_lim = len - 1;        // last visible key of the row, and the least of the tile's
     {
       const int per = p.tile_pos * p.q.group;    // rows of a sequence in the tile
@@ -513,7 +519,10 @@ attn_rows_kernel(const __grid_constant__ RowsMaps maps, const RowsParams p) {
       const int first_pos = p.pos_tiles == 1 ? 0 : tile % p.pos_tiles * p.tile_pos;
       const int pos = first_pos + r_in_tile % per / p.q.group;
       live = live && i < p.s.n && pos < p.q.Sq;
-      number = (static_cast<int64_t>(seq * p.s.n + i) * p.q.Sq + pos) * p.q.H + hk * p.q.group + r_in_tile % p.q.group;
+      const int64_t b = seq * p.s.n + i, h = hk * p.q.group + r_in_tile % p.q.group;
+      number = (b * p.q.Sq + pos) * p.q.H + h;
+      out_at = b * p.o_sb + pos * p.o_ss + h * p.o_sh;
+      lse_at = (b * p.q.H + h) * p.q.Sq + pos;
       if (p.s.causal) {
         lim = min(lim, pos + len - p.q.Sq);
         min_lim = min(min_lim, first_pos + len - p.q.Sq);
@@ -647,62 +656,117 @@ attn_rows_kernel(const __grid_constant__ RowsMaps maps, const RowsParams p) {
     // ---- the part's results: unnormalised O, reference, sum
     if (l == 0.f) m_ref = -INFINITY;                // (nothing seen)
     else if (!(m_ref > -INFINITY)) m_ref = 0.f;     // (nothing but NaN: the sum)
-    float* orow = p.mine.o + (number * p.mine.parts + part) * 128;
-    float2* ml = reinterpret_cast<float2*>(p.mine.ml) + number * p.mine.parts + part;
-    if constexpr (kPair) {
-      if (live) *ml = make_float2(m_ref, l);
-      if (n_t > 0) {
+    if constexpr (!kFinish) {
+      float* orow = p.mine.o + (number * p.mine.parts + part) * 128;
+      float2* ml = reinterpret_cast<float2*>(p.mine.ml) + number * p.mine.parts + part;
+      if constexpr (kPair) {
+        if (live) *ml = make_float2(m_ref, l);
+        if (n_t > 0) {
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          uint32_t o[32];
-          tmem_ld32(tO + c * 32, o);
-          tmem_wait_ld();
-          if (live) {
+          for (int c = 0; c < 4; ++c) {
+            uint32_t o[32];
+            tmem_ld32(tO + c * 32, o);
+            tmem_wait_ld();
+            if (live) {
 #pragma unroll
-            for (int g = 0; g < 4; ++g) st_global_v8(orow + c * 32 + g * 8, &o[g * 8]);
+              for (int g = 0; g < 4; ++g) st_global_v8(orow + c * 32 + g * 8, &o[g * 8]);
+            }
+          }
+        }
+      } else {
+        // the slots' factors to a common reference; each writes half of the columns
+        // (every softmax warp gets to the barriers, expired waits or not)
+        if (t == 1) row_s[r_in_tile] = make_float2(m_ref, l);
+        tc_fence_before_sync();
+        named_bar_sync(1, 256);
+        float f0, f1;
+        if (t == 0) {
+          const float2 o = row_s[r_in_tile];
+          const float mm = fmaxf(m_ref, o.x);
+          f0 = m_ref > -INFINITY ? ex2(m_ref - mm) : 0.f;
+          f1 = o.x > -INFINITY ? ex2(o.x - mm) : 0.f;
+          row_s[r_in_tile] = make_float2(f0, f1);
+          if (live) *ml = make_float2(mm, fmaf(f1, o.y, f0 * l));
+        }
+        named_bar_sync(1, 256);
+        tc_fence_after_sync();
+        if (t == 1) {
+          f0 = row_s[r_in_tile].x;
+          f1 = row_s[r_in_tile].y;
+        }
+        const uint32_t tA = tbase + lane_base + 256 + t * 64;
+        if (n > 0) {
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            uint32_t o0[32], o1[32];
+            tmem_ld32(tA + c * 32, o0);
+            if (n1 > 0) tmem_ld32(tA + 128 + c * 32, o1);
+            tmem_wait_ld();
+#pragma unroll
+            for (int i = 0; i < 32; ++i) {
+              float y = __uint_as_float(o0[i]) * f0;
+              if (n1 > 0) y = fmaf(__uint_as_float(o1[i]), f1, y);
+              o0[i] = __float_as_uint(y);
+            }
+            if (live) {
+#pragma unroll
+              for (int g = 0; g < 4; ++g) st_global_v8(orow + t * 64 + c * 32 + g * 8, &o0[g * 8]);
+            }
           }
         }
       }
     } else {
-      // the slots' factors to a common reference; each writes half of the columns
-      // (every softmax warp gets to the barriers, expired waits or not)
-      if (t == 1) row_s[r_in_tile] = make_float2(m_ref, l);
-      tc_fence_before_sync();
-      named_bar_sync(1, 256);
-      float f0, f1;
-      if (t == 0) {
-        const float2 o = row_s[r_in_tile];
-        const float mm = fmaxf(m_ref, o.x);
-        f0 = m_ref > -INFINITY ? ex2(m_ref - mm) : 0.f;
-        f1 = o.x > -INFINITY ? ex2(o.x - mm) : 0.f;
-        row_s[r_in_tile] = make_float2(f0, f1);
-        if (live) *ml = make_float2(mm, fmaf(f1, o.y, f0 * l));
-      }
-      named_bar_sync(1, 256);
-      tc_fence_after_sync();
-      if (t == 1) {
-        f0 = row_s[r_in_tile].x;
-        f1 = row_s[r_in_tile].y;
-      }
-      const uint32_t tA = tbase + lane_base + 256 + t * 64;
-      if (n > 0) {
+      // 32 columns from `col` on, zeros where nothing was seen
+      auto put = [&](const float (&o)[32], int col) {
+        if (!live) return;
+        uint32_t w[16];
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          uint32_t o0[32], o1[32];
-          tmem_ld32(tA + c * 32, o0);
-          if (n1 > 0) tmem_ld32(tA + 128 + c * 32, o1);
-          tmem_wait_ld();
+        for (int i = 0; i < 16; ++i) w[i] = pack2<kBF16>(o[2 * i], o[2 * i + 1]);
 #pragma unroll
-          for (int i = 0; i < 32; ++i) {
-            float y = __uint_as_float(o0[i]) * f0;
-            if (n1 > 0) y = fmaf(__uint_as_float(o1[i]), f1, y);
-            o0[i] = __float_as_uint(y);
-          }
-          if (live) {
-#pragma unroll
-            for (int g = 0; g < 4; ++g) st_global_v8(orow + t * 64 + c * 32 + g * 8, &o0[g * 8]);
-          }
+        for (int i = 0; i < 4; ++i)
+          *reinterpret_cast<uint4*>(p.out + out_at + col + 8 * i) = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+      };
+      float f0 = l == 0.f ? 0.f : 1.f / l, f1 = 0.f, ref = m_ref, sum = l;
+      if constexpr (!kPair) {
+        if (t == 1) row_s[r_in_tile] = make_float2(m_ref, l);
+        tc_fence_before_sync();
+        named_bar_sync(1, 256);
+        if (t == 0) {
+          const float2 o = row_s[r_in_tile];
+          ref = fmaxf(m_ref, o.x);
+          f0 = m_ref > -INFINITY ? ex2(m_ref - ref) : 0.f;
+          f1 = o.x > -INFINITY ? ex2(o.x - ref) : 0.f;
+          sum = fmaf(f1, o.y, f0 * l);
+          const float inv = sum == 0.f ? 0.f : 1.f / sum;
+          f0 *= inv;
+          f1 *= inv;
+          row_s[r_in_tile] = make_float2(f0, f1);
         }
+        named_bar_sync(1, 256);
+        tc_fence_after_sync();
+        if (t == 1) {
+          f0 = row_s[r_in_tile].x;
+          f1 = row_s[r_in_tile].y;
+        }
+      }
+      if (live && p.lse2 != nullptr && (kPair || t == 0)) p.lse2[lse_at] = ref + log2f(sum);
+      // (two tiles: a slot's own 128 columns; one: half of both accumulators')
+      const uint32_t tA = kPair ? tO : tbase + lane_base + 256 + t * 64;
+#pragma unroll
+      for (int c = 0; c < (kPair ? 4 : 2); ++c) {
+        uint32_t o0[32], o1[32];
+        float y[32];
+        if (n > 0) {
+          tmem_ld32(tA + c * 32, o0);
+          if (!kPair && n1 > 0) tmem_ld32(tA + 128 + c * 32, o1);
+          tmem_wait_ld();
+        }
+#pragma unroll
+        for (int i = 0; i < 32; ++i) {
+          y[i] = n > 0 ? __uint_as_float(o0[i]) * f0 : 0.f;
+          if (!kPair && n1 > 0) y[i] = fmaf(__uint_as_float(o1[i]), f1, y[i]);
+        }
+        put(y, kPair ? c * 32 : t * 64 + c * 32);
       }
     }
   }
@@ -713,6 +777,7 @@ attn_rows_kernel(const __grid_constant__ RowsMaps maps, const RowsParams p) {
     __syncwarp();
     tmem_dealloc(tbase, 512);
   }
+  if (p.chained) griddep_wait();
 }
 
 // ---- merge: parts in the order of the keys -------------------------------------------------------------
@@ -862,7 +927,7 @@ Tiles tiles_of(const Segment& s, const RowShape& q) {
   return t;
 }
 
-template <bool kBF16, int kFmt, bool kPair>
+template <bool kBF16, int kFmt, bool kPair, bool kFinish>
 cudaError_t launch_rows_of(const CacheRows& c, const CacheAttnArgs& a, RowsParams& p, const Tiles& tiles, cudaStream_t stream) {
   using C = Cfg<kFmt, kPair>;
   RowsMaps maps;
@@ -877,7 +942,7 @@ cudaError_t launch_rows_of(const CacheRows& c, const CacheAttnArgs& a, RowsParam
   } else {
     maps.ks = maps.vs = maps.k;
   }
-  const auto kern = attn_rows_kernel<kBF16, kFmt, kPair>;
+  const auto kern = attn_rows_kernel<kBF16, kFmt, kPair, kFinish>;
   cudaError_t e = ensure_dynamic_smem(reinterpret_cast<const void*>(kern), C::kSmem);
   if (e != cudaSuccess) return e;
   e = check_register_budget(reinterpret_cast<const void*>(kern), C::kThreads, C::kBlockRegs);
@@ -890,8 +955,11 @@ cudaError_t launch_rows_of(const CacheRows& c, const CacheAttnArgs& a, RowsParam
 
 template <bool kBF16, int kFmt>
 cudaError_t launch_rows_fmt(const CacheRows& c, const CacheAttnArgs& a, RowsParams& p, const Tiles& tiles, cudaStream_t stream) {
-  return tiles.count > 1 ? launch_rows_of<kBF16, kFmt, true>(c, a, p, tiles, stream)
-                         : launch_rows_of<kBF16, kFmt, false>(c, a, p, tiles, stream);
+  if (p.out != nullptr)
+    return tiles.count > 1 ? launch_rows_of<kBF16, kFmt, true, true>(c, a, p, tiles, stream)
+                           : launch_rows_of<kBF16, kFmt, false, true>(c, a, p, tiles, stream);
+  return tiles.count > 1 ? launch_rows_of<kBF16, kFmt, true, false>(c, a, p, tiles, stream)
+                         : launch_rows_of<kBF16, kFmt, false, false>(c, a, p, tiles, stream);
 }
 
 }  // namespace
@@ -915,7 +983,7 @@ int attn_rows_parts(const Segment& s, const RowShape& q, int num_sms) {
 }
 
 cudaError_t launch_attn_rows(const CacheRows& c, const Segment& s, const CacheAttnArgs& a, const Partials& mine,
-                             cudaStream_t stream) {
+                             bool finish, bool chained, cudaStream_t stream) {
   RowsParams p;
   p.s = s;
   p.q = RowShape{a.Sq, a.H, a.H / a.group, a.group};
@@ -928,6 +996,10 @@ cudaError_t launch_attn_rows(const CacheRows& c, const Segment& s, const CacheAt
   p.parts = mine.parts;
   p.scale_log2 = a.softmax_scale * 1.4426950408889634f;
   p.mine = mine;
+  p.out = finish ? a.out : nullptr;
+  p.o_sb = a.o_sb; p.o_ss = a.o_ss; p.o_sh = a.o_sh;
+  p.lse2 = a.lse2;
+  p.chained = chained ? 1 : 0;
   p.status = device_status_words();
   if (a.bf16) {
     if (c.format == CACHE_I8) return launch_rows_fmt<true, CACHE_I8>(c, a, p, tiles, stream);
