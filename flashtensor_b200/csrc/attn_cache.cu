@@ -17,6 +17,8 @@
 //     the weights get from one to the other by transposing 8x8 blocks between registers;
 //   - a unit that lies in one range is finished there; what a range has of a unit that others share goes to the workspace
 //     and is merged by attn_merge_kernel in the order of the keys, so results do not depend on which warp was first.
+// Small calls are bound by the launches and by one unit's latency, not by bytes: there a cluster of up to eight CTAs takes a unit, its warps
+// an equal range each, and merges through its distributed shared memory (see `cluster_of`); there is no deal, workspace or second launch.
 // Codes of 8 bits go from shared memory straight into matrix fragments:
 //   - codes become f16, exactly (int8 as the low bits of 1024 + 128 + code, less 1152; e4m3 by conversion), and q is brought
 //     to f16 too, a bf16 row times the power of two that puts its largest value in [1, 2): what is lost is below 2^-24 of it;
@@ -38,6 +40,8 @@ constexpr int kWarps = 12;   // workers of a CTA, one CTA to an SM
 constexpr int kStages = 2;   // of each worker's ring
 constexpr int kThreads = kWarps * 32;
 constexpr int kMinTiles = 2;  // a worker's share is no less
+constexpr int kMaxCluster = 8;  // CTAs to a unit
+constexpr int kFewTiles = 10;  // of a warp of the cluster form, at most
 template <int kFmt> struct Tile {
   static constexpr int kKeys = kFmt == CACHE_16 ? 16 : 32;
   static constexpr uint32_t kHalf = 2048;                  // (16 bits) one 64-column half of the keys or values
@@ -86,6 +90,26 @@ __device__ __forceinline__ int64_t quotient(int64_t x, int64_t y) {
   if (static_cast<uint64_t>(x | y) >> 32 == 0) return static_cast<uint32_t>(x) / static_cast<uint32_t>(y);
   return x / y;
 }
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ uint32_t cluster_size() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ float ld_cluster(uint32_t smem_addr, uint32_t rank) {
+  uint32_t remote;
+  float v;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(smem_addr), "r"(rank));
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(remote) : "memory");
+  return v;
+}
 // an 8x8 block of 16-bit values, rows and columns exchanged
 __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
   uint32_t y;
@@ -110,7 +134,9 @@ struct Cursor {
 };
 
 // One CTA to an SM; a warp is a worker.  kOct: eights of query rows to a unit.
-template <bool kBF16, int kFmt, int kOct>
+// kCluster: few units and few keys.  A unit is a cluster of CTAs, whose warps share its tiles and whose results are merged through
+// distributed shared memory, in the order of the keys' owners: no second launch, and no deal.
+template <bool kBF16, int kFmt, int kOct, bool kCluster>
 __global__ void __launch_bounds__(kThreads, 1)
 attn_stream_kernel(const __grid_constant__ StreamMaps maps, const StreamParams p) {
   using T = Tile<kFmt>;
@@ -119,6 +145,9 @@ attn_stream_kernel(const __grid_constant__ StreamMaps maps, const StreamParams p
   extern __shared__ uint8_t smem_raw[];
   __shared__ __align__(8) uint64_t full[kWarps][kStages];
   __shared__ uint32_t abort_s;
+  __shared__ float2 ml_s[kCluster ? kWarps : 1][8 * kOct];    // (kCluster) every warp's reference and sum of every row
+  __shared__ float cta_o[kCluster ? 8 * kOct : 1][128];       // the CTA's results, read by the whole cluster
+  __shared__ float2 cta_ml[8 * kOct];
 
   const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -149,47 +178,58 @@ attn_stream_kernel(const __grid_constant__ StreamMaps maps, const StreamParams p
     c.len = seen_of(p.s[c.seg], c.seq);
     c.tiles = (c.len + T::kKeys - 1) / T::kKeys;
   };
-  const int per = (n_seqs + 31) / 32;
-  int64_t upto = 0;
-#pragma unroll 4
-  for (int i = lane * per; i < min(n_seqs, (lane + 1) * per); ++i) {
-    Cursor c;
-    at(i, c);
-    upto += c.tiles;
-  }
-#pragma unroll
-  for (int d = 1; d < 32; d <<= 1) {
-    const int64_t x = __shfl_up_sync(0xffffffffu, upto, d);
-    if (lane >= d) upto += x;
-  }
-  upto *= p.q.Hkv;  // tiles of this lane's sequences and those before
-  const int64_t total = __shfl_sync(0xffffffffu, upto, 31);
-  const int64_t workers = static_cast<int64_t>(gridDim.x) * kWarps;
-  const int64_t share = max(static_cast<int64_t>(quotient(total + workers - 1, workers)), static_cast<int64_t>(kMinTiles));
-
-  // (neighbours in the numbering on different SMs, so that a small launch uses all of them)
-  const int64_t worker = static_cast<int64_t>(warp) * gridDim.x + blockIdx.x;
-  const int64_t lo = worker * share;
-  const int count = static_cast<int>(min(share, total - lo));  // (a worker's tiles are 8 KB each: far below 2^31)
-  if (count <= 0) {
-    if (p.chained) griddep_wait();
-    return;
-  }
-
+  int64_t worker = 0, share = 0;
+  int count;
   Cursor c;
-  {
-    const int x = __ffs(__ballot_sync(0xffffffffu, upto > lo)) - 1;  // the lane whose sequences the range begins in
-    int64_t rest = lo - (x > 0 ? __shfl_sync(0xffffffffu, upto, max(x - 1, 0)) : 0);
-    for (int i = x * per;; ++i) {  // (bounded, should another stream change the lengths in between)
+  if constexpr (kCluster) {
+    const int unit = static_cast<int>(blockIdx.x / cluster_size());
+    at(unit / p.q.Hkv, c);
+    c.hk = unit % p.q.Hkv;
+    const int each = max((c.tiles + static_cast<int>(cluster_size()) * kWarps - 1) / (static_cast<int>(cluster_size()) * kWarps), 1);
+    c.tile = (warp * static_cast<int>(cluster_size()) + static_cast<int>(cluster_rank())) * each;
+    count = max(min(each, c.tiles - c.tile), 0);
+  } else {
+    const int per = (n_seqs + 31) / 32;
+    int64_t upto = 0;
+#pragma unroll 4
+    for (int i = lane * per; i < min(n_seqs, (lane + 1) * per); ++i) {
+      Cursor c;
       at(i, c);
-      const int64_t in_seq = static_cast<int64_t>(c.tiles) * p.q.Hkv;
-      if (rest < in_seq || i + 1 == n_seqs) break;
-      rest -= in_seq;
+      upto += c.tiles;
     }
-    c.tiles = max(c.tiles, 1);
-    const int64_t hk = quotient(rest, c.tiles);
-    c.hk = static_cast<int>(min(hk, static_cast<int64_t>(p.q.Hkv - 1)));
-    c.tile = static_cast<int>(min(rest - hk * c.tiles, static_cast<int64_t>(c.tiles - 1)));
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int64_t x = __shfl_up_sync(0xffffffffu, upto, d);
+      if (lane >= d) upto += x;
+    }
+    upto *= p.q.Hkv;  // tiles of this lane's sequences and those before
+    const int64_t total = __shfl_sync(0xffffffffu, upto, 31);
+    const int64_t workers = static_cast<int64_t>(gridDim.x) * kWarps;
+    share = max(static_cast<int64_t>(quotient(total + workers - 1, workers)), static_cast<int64_t>(kMinTiles));
+
+    // (neighbours in the numbering on different SMs, so that a small launch uses all of them)
+    worker = static_cast<int64_t>(warp) * gridDim.x + blockIdx.x;
+    const int64_t lo = worker * share;
+    count = static_cast<int>(min(share, total - lo));  // (a worker's tiles are 8 KB each: far below 2^31)
+    if (count <= 0) {
+      if (p.chained) griddep_wait();
+      return;
+    }
+
+    {
+      const int x = __ffs(__ballot_sync(0xffffffffu, upto > lo)) - 1;  // the lane whose sequences the range begins in
+      int64_t rest = lo - (x > 0 ? __shfl_sync(0xffffffffu, upto, max(x - 1, 0)) : 0);
+      for (int i = x * per;; ++i) {  // (bounded, should another stream change the lengths in between)
+        at(i, c);
+        const int64_t in_seq = static_cast<int64_t>(c.tiles) * p.q.Hkv;
+        if (rest < in_seq || i + 1 == n_seqs) break;
+        rest -= in_seq;
+      }
+      c.tiles = max(c.tiles, 1);
+      const int64_t hk = quotient(rest, c.tiles);
+      c.hk = static_cast<int>(min(hk, static_cast<int64_t>(p.q.Hkv - 1)));
+      c.tile = static_cast<int>(min(rest - hk * c.tiles, static_cast<int64_t>(c.tiles - 1)));
+    }
   }
   auto advance = [&](Cursor& x) {  // (only where a tile follows)
     if (++x.tile < x.tiles) return;
@@ -242,7 +282,7 @@ attn_stream_kernel(const __grid_constant__ StreamMaps maps, const StreamParams p
 
   Cursor ahead = c;  // the next tile to fetch
   int fetched = 0;
-  prefetch_rows(c);
+  if (count > 0) prefetch_rows(c);
 #pragma unroll
   for (int i = 0; i < kStages; ++i) {
     if (i >= count) continue;
@@ -317,7 +357,7 @@ attn_stream_kernel(const __grid_constant__ StreamMaps maps, const StreamParams p
         for (int i = 0; i < 8; ++i) o[y][i][0] = o[y][i][1] = o[y][i][2] = o[y][i][3] = 0.f;
       }
       min_lim = s.causal ? min(c.len - 1, c.len - p.q.Sq) : c.len - 1;
-      if (first == 0 && lane == 0) {
+      if (!kCluster && first == 0 && lane == 0) {
         const int rest = c.tiles - (count - n);  // behind this worker's range
         p.deal[c.seg].workers[static_cast<int64_t>(c.seq) * p.q.Hkv + c.hk] =
             make_int2(static_cast<int>(worker), static_cast<int>(worker + (rest > 0 ? quotient(rest + share - 1, share) : 0)));
@@ -518,7 +558,7 @@ attn_stream_kernel(const __grid_constant__ StreamMaps maps, const StreamParams p
       if (fetched < count) advance(ahead);
     }
 
-    if (c.tile + 1 == c.tiles || n + 1 == count) {
+    if (!kCluster && (c.tile + 1 == c.tiles || n + 1 == count)) {
       // ---- the unit ends, or this range of it
       const Segment& sg = p.s[c.seg];
       const bool whole = first == 0 && c.tile + 1 == c.tiles;
@@ -588,10 +628,91 @@ attn_stream_kernel(const __grid_constant__ StreamMaps maps, const StreamParams p
       mbar_wait(smem_u32(&full[warp][n % kStages]), (n / kStages) & 1, &none);
   }
   if (p.chained) griddep_wait();
+  if constexpr (kCluster) {
+    // ---- the warps' results, one CTA's, the cluster's; a ring whose tiles are all used holds its warp's
+    const Segment& sg = p.s[0];
+    float* results = reinterpret_cast<float*>(smem_raw + (smem_base - smem_u32(smem_raw)));
+    float* mine = results + warp * (kStages * kTileBytes / 4);
+#pragma unroll
+    for (int y = 0; y < kOct; ++y) {
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        const int r = 8 * y + 2 * t4 + x;
+        float sum = count > 0 ? l[y][x] : 0.f;
+        sum += __shfl_xor_sync(0xffffffffu, sum, 4);
+        sum += __shfl_xor_sync(0xffffffffu, sum, 8);
+        sum += __shfl_xor_sync(0xffffffffu, sum, 16);
+        if (r0 == 0) ml_s[warp][r] = make_float2(count > 0 ? m[y][x] : -INFINITY, sum);
+        if (count <= 0 || r >= sg.rows) continue;
+        if constexpr (k8) {
+#pragma unroll
+          for (int i = 0; i < 8; i += 2)
+            *reinterpret_cast<float4*>(mine + r * 128 + 16 * r0 + 2 * i) = make_float4(o[y][i][x], o[y][i][2 + x], o[y][i + 1][x], o[y][i + 1][2 + x]);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            mine[r * 128 + 16 * i + r0] = o[y][i][x];
+            mine[r * 128 + 16 * i + 8 + r0] = o[y][i][2 + x];
+          }
+        }
+      }
+    }
+    __syncthreads();
+    const int cols = tid & 127;  // three rows at a time, a thread to a column
+    for (int r = tid >> 7; r < sg.rows; r += kThreads / 128) {
+      float top = -INFINITY, sum = 0.f, acc = 0.f;
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) top = fmaxf(top, ml_s[w][r].x);
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) {
+        const float2 ml = ml_s[w][r];
+        if (ml.x > -INFINITY || ml.y != 0.f) {  // (else nothing seen; nothing but NaN: the sum)
+          const float f = ml.x > -INFINITY ? ex2(ml.x - top) : 1.f;
+          sum = fmaf(f, ml.y, sum);
+          acc = fmaf(f, results[w * (kStages * kTileBytes / 4) + r * 128 + cols], acc);
+        }
+      }
+      cta_o[r][cols] = acc;
+      if (cols == 0) cta_ml[r] = make_float2(top, sum);
+    }
+    cluster_sync();
+    const int parts = static_cast<int>(cluster_size());
+    for (int r = static_cast<int>(cluster_rank()) + parts * (tid >> 7); r < sg.rows; r += parts * (kThreads / 128)) {
+      float2 ml[kMaxCluster];
+      float po[kMaxCluster];
+      float top = -INFINITY, sum = 0.f, acc = 0.f;
+#pragma unroll
+      for (int x = 0; x < kMaxCluster; ++x) {
+        if (x >= parts) continue;
+        ml[x].x = ld_cluster(smem_u32(&cta_ml[r].x), x);
+        ml[x].y = ld_cluster(smem_u32(&cta_ml[r].y), x);
+        po[x] = ld_cluster(smem_u32(&cta_o[r][cols]), x);
+      }
+#pragma unroll
+      for (int x = 0; x < kMaxCluster; ++x)
+        if (x < parts) top = fmaxf(top, ml[x].x);
+#pragma unroll
+      for (int x = 0; x < kMaxCluster; ++x) {
+        if (x < parts && (ml[x].x > -INFINITY || ml[x].y != 0.f)) {
+          const float f = ml[x].x > -INFINITY ? ex2(ml[x].x - top) : 1.f;
+          sum = fmaf(f, ml[x].y, sum);
+          acc = fmaf(f, po[x], acc);
+        }
+      }
+      const Row row = decode_row(r, c.seq, c.hk, sg, p.q);
+      const float y = sum == 0.f ? 0.f : acc / sum;
+      const float next = __shfl_down_sync(0xffffffffu, y, 1);
+      if ((cols & 1) == 0)
+        *reinterpret_cast<uint32_t*>(p.out + row.b * p.o_sb + row.pos * p.o_ss + row.h * p.o_sh + cols) = pack2<kBF16>(y, next);
+      if (p.lse2 != nullptr && cols == 0)
+        p.lse2[(static_cast<int64_t>(row.b) * p.q.H + row.h) * p.q.Sq + row.pos] = top + log2f(sum);
+    }
+    cluster_sync();  // no CTA leaves while another still reads its shared memory
+  }
 }
 
 template <int kFmt>
-cudaError_t launch_stream_fmt(const CacheRows* const* c, StreamParams& p, bool bf16, int num_sms, cudaStream_t stream) {
+cudaError_t launch_stream_fmt(const CacheRows* const* c, StreamParams& p, bool bf16, int cluster, int num_sms, cudaStream_t stream) {
   using T = Tile<kFmt>;
   StreamMaps maps;
   for (int x = 0; x < 2; ++x) {
@@ -609,8 +730,18 @@ cudaError_t launch_stream_fmt(const CacheRows* const* c, StreamParams& p, bool b
   const uint32_t smem = kWarps * kStages * kTileBytes + 1024;
   bool wide = false;
   for (int x = 0; x < p.segments; ++x) wide = wide || p.s[x].rows > 8;
-  const auto kern = bf16 ? (wide ? attn_stream_kernel<true, kFmt, 2> : attn_stream_kernel<true, kFmt, 1>)
-                         : (wide ? attn_stream_kernel<false, kFmt, 2> : attn_stream_kernel<false, kFmt, 1>);
+  if (cluster > 0) {
+    const auto kern = bf16 ? (wide ? attn_stream_kernel<true, kFmt, 2, true> : attn_stream_kernel<true, kFmt, 1, true>)
+                           : (wide ? attn_stream_kernel<false, kFmt, 2, true> : attn_stream_kernel<false, kFmt, 1, true>);
+    cudaError_t e = ensure_dynamic_smem(reinterpret_cast<const void*>(kern), smem);
+    if (e != cudaSuccess) return e;
+    e = launch_dependent_cluster(kern, dim3(static_cast<unsigned>(p.s[0].N * p.q.Hkv * cluster)), dim3(kThreads), smem,
+                                 static_cast<unsigned>(cluster), stream, maps, p);
+    count_launch();
+    return e;
+  }
+  const auto kern = bf16 ? (wide ? attn_stream_kernel<true, kFmt, 2, false> : attn_stream_kernel<true, kFmt, 1, false>)
+                         : (wide ? attn_stream_kernel<false, kFmt, 2, false> : attn_stream_kernel<false, kFmt, 1, false>);
   cudaError_t e = ensure_dynamic_smem(reinterpret_cast<const void*>(kern), smem);
   if (e != cudaSuccess) return e;
   e = launch_dependent(kern, dim3(static_cast<unsigned>(num_sms)), dim3(kThreads), smem, stream, maps, p);
@@ -618,26 +749,45 @@ cudaError_t launch_stream_fmt(const CacheRows* const* c, StreamParams& p, bool b
   return e;
 }
 
-cudaError_t launch_stream(const CacheRows* const* c, StreamParams& p, bool bf16, int num_sms, cudaStream_t stream) {
+cudaError_t launch_stream(const CacheRows* const* c, StreamParams& p, bool bf16, int cluster, int num_sms, cudaStream_t stream) {
   switch (c[0]->format) {
-    case CACHE_I8: return launch_stream_fmt<CACHE_I8>(c, p, bf16, num_sms, stream);
-    case CACHE_E4M3: return launch_stream_fmt<CACHE_E4M3>(c, p, bf16, num_sms, stream);
-    default: return launch_stream_fmt<CACHE_16>(c, p, bf16, num_sms, stream);
+    case CACHE_I8: return launch_stream_fmt<CACHE_I8>(c, p, bf16, cluster, num_sms, stream);
+    case CACHE_E4M3: return launch_stream_fmt<CACHE_E4M3>(c, p, bf16, cluster, num_sms, stream);
+    default: return launch_stream_fmt<CACHE_16>(c, p, bf16, cluster, num_sms, stream);
   }
 }
 
 // Which kernel takes a segment of up to 16 rows to a unit; the other one's tiles (attn_rows.cu) are mostly empty then, but
 // 16-bit keys come in copies four times as large and need no instruction of a warp.  It has a CTA for a unit, or several,
-// and nothing to follow a short one; the stream is even whatever the units are.  Streamed / tiles, us:
-//   16 bits, 4 rows   8 units 1024 keys 8.7/7.7, 8000 keys 17.7/14.6; 32 units 4001 keys 18.1/16.6, 128 units 43.8/41.4;
+// and nothing to follow a short one; the stream is even whatever the units are.  Dealt out / tiles, us:
+//   16 bits, 4 rows   8 units 8000 keys 17.7/14.6; 32 units 4001 keys 18.1/16.6, 128 units 43.8/41.4;
 //                     128 units 16384 keys 140/135; 256 units 1000 keys 26.6/28.4, 512 units 500 keys 26.7/39.4
 //   16 bits, 16 rows  16 units 8003 keys 25.3/17.2, 128 units 4001 keys 52/43
-//   8 bits, 4 rows    8 units 1024 keys 8.4/8.6, 8000 keys 13.7/15.0; 128 units 4001 keys 30.6/57.8
+//   8 bits, 4 rows    8 units 8000 keys 13.7/15.0; 128 units 4001 keys 30.6/57.8
 //   8 bits, 16 rows   16 units 8003 keys 26/20; 8 units 32000 keys 34/37; 128 units 4001 keys 44/58
 bool streams(const Segment& s, const RowShape& q, int format, int num_sms) {
   if (s.rows > kRows) return false;
   const int64_t units = static_cast<int64_t>(s.N) * q.Hkv;
   return format == CACHE_16 ? units > num_sms : s.rows <= 8 || 4 * units > num_sms;
+}
+
+// CTAs of a cluster for each unit of a lone segment, or 0 for none.  The cluster form is one launch and has no deal, 2.5 us less, and costs
+// what a unit's warps have more tiles to do (2 us each) than an even share.  Clusters / the form that `streams` chooses, us, 4 rows,
+// 8 heads, sequences of half to all of the longest:
+//   8 bits   B1 1000 keys 5.9/8.6, 4000 7.9/11.1, 16000 16.7/18.5; B4 1000 6.4/9.2, 4000 12.2/15.1, 16000 28.4/28.1;
+//            B16 1000 12.7/16.1, 4000 28.7/29.1; B2 16000 with four CTAs 25.6/20.6
+//   16 bits  B1 1000 keys 6.5/7.8, 4000 10.2/12.7, 16000 23.8/17.3; B4 1000 8.5/10.3, 4000 15.2/16.9; B16 1000 15.2/15.1, 4000 43/39
+// Of clusters of eight only some fit at once: 8 bits, B2 4000 keys, 16 units, 14.8 with eight CTAs to each, 10.9 with four.
+int cluster_of(const Segment& s, const RowShape& q, int format, int num_sms) {
+  if (s.rows > (format == CACHE_16 ? 8 : kRows)) return 0;
+  const int64_t units = static_cast<int64_t>(s.N) * q.Hkv;
+  const int keys = format == CACHE_16 ? Tile<CACHE_16>::kKeys : Tile<CACHE_I8>::kKeys, tiles = (s.S + keys - 1) / keys;
+  int parts = 1;
+  while (parts < kMaxCluster && units * parts * 2 <= (parts == kMaxCluster / 2 ? 2 * num_sms / 3 : num_sms) && tiles > parts * kWarps)
+    parts *= 2;
+  const int64_t each = (tiles + parts * kWarps - 1) / (parts * kWarps), workers = static_cast<int64_t>(num_sms) * kWarps;
+  const int64_t share = (units * tiles + workers - 1) / workers;
+  return units * parts <= num_sms && each <= kFewTiles && each <= (share > kMinTiles ? share : kMinTiles) + 3 ? parts : 0;
 }
 
 size_t row_count(const CacheAttnArgs& a) { return static_cast<size_t>(a.B) * a.Sq * a.H; }
@@ -661,6 +811,7 @@ struct Plan {
   const CacheRows* c[2];
   bool have[2], stream[2], together;
   bool finished;       // the own rows' kernel leaves nothing to merge
+  int cluster;         // CTAs to a unit of the stream's cluster form, 0: dealt out
   Source from[2];      // partial results
   size_t bytes;
 };
@@ -679,6 +830,8 @@ Plan plan_of(const CacheAttnArgs& a, void* ws, int num_sms) {
     x.stream[i] = streams(x.s[i], q, x.c[i]->format, num_sms);
   }
   x.finished = false;
+  x.cluster = x.have[0] ? 0 : cluster_of(x.s[1], q, a.own.format, num_sms);
+  if (x.cluster > 0) x.stream[1] = true;
   x.together = x.stream[0] && x.stream[1] && a.prefix.format == a.own.format;
   Carver w{static_cast<uint8_t*>(ws), 0};
   const size_t rows = row_count(a), workers = static_cast<size_t>(num_sms) * kWarps;
@@ -693,6 +846,10 @@ Plan plan_of(const CacheAttnArgs& a, void* ws, int num_sms) {
       if (x.finished) continue;
       f.fixed.o = w.take<float>(rows * f.fixed.parts * 128);
       f.fixed.ml = w.take<float>(rows * f.fixed.parts * 2);
+      continue;
+    }
+    if (x.cluster > 0) {
+      x.finished = true;
       continue;
     }
     Dealt& d = f.deal;
@@ -744,7 +901,7 @@ cudaError_t launch_attn_cache(const CacheAttnArgs& a, void* ws, int num_sms, cud
         p.s[y] = x.s[i + y];
         p.deal[y] = x.from[i + y].deal;
       }
-      e = launch_stream(x.c + i, p, a.bf16, num_sms, stream);
+      e = launch_stream(x.c + i, p, a.bf16, x.cluster, num_sms, stream);
     } else {
       e = launch_attn_rows(*x.c[i], x.s[i], a, x.from[i].fixed, x.finished, chained, stream);
     }

@@ -319,6 +319,24 @@ def test_attention_over_ragged_caches(ops, shape, fmt, dtype):
   assert same(ft().CacheAttn(Hkv, H).forward(q, cache, n), ops.attn_cache(q, cache, n))
 
 
+# many units and few, of one part or several: B, Sq, H, Hkv, capacity
+UNITS = [(150, 1, 2, 1, 70), (400, 1, 4, 1, 40), (100, 2, 8, 4, 90), (75, 4, 16, 2, 300), (60, 4, 16, 4, 100), (20, 4, 16, 4, 800),
+         (100, 20, 2, 1, 500), (20, 70, 8, 4, 333), (40, 1, 24, 1, 1700), (9, 1, 16, 8, 1500), (3, 1, 8, 8, 4000), (1, 1, 8, 8, 16000),
+         (2, 1, 16, 2, 30000), (1, 2, 5, 5, 20000)]
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("fmt", [None] + FORMATS, ids=str)
+@pytest.mark.parametrize("shape", UNITS, ids=str)
+def test_attention_of_many_and_few_units(ops, shape, fmt, dtype):
+  B, Sq, H, Hkv, cap = shape
+  cache = make_cache(B, cap, Hkv, fmt or dtype, 160, dtype)
+  lens = [0 if i % 7 == 3 else cap - 13 * i % cap for i in range(B)]
+  q, n = q_of(B, Sq, H, dtype, 161, 1.5), ints(lens)
+  got, lse = ops.attn_cache(q, cache, kv_len=n, return_lse=True)
+  check_attention(got, lse, _attention(q, cache, lens), "")
+
+
 @pytest.mark.parametrize("fmt", [None] + FORMATS, ids=str)
 @pytest.mark.parametrize("Sq, group", [(1, 4), (4, 1), (9, 4)])
 def test_attention_without_lengths_and_with_a_scale(ops, fmt, Sq, group):
