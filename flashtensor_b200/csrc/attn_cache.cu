@@ -731,8 +731,9 @@ cudaError_t launch_stream_fmt(const CacheRows* const* c, StreamParams& p, bool b
   bool wide = false;
   for (int x = 0; x < p.segments; ++x) wide = wide || p.s[x].rows > 8;
   if (cluster > 0) {
-    const auto kern = bf16 ? (wide ? attn_stream_kernel<true, kFmt, 2, true> : attn_stream_kernel<true, kFmt, 1, true>)
-                           : (wide ? attn_stream_kernel<false, kFmt, 2, true> : attn_stream_kernel<false, kFmt, 1, true>);
+    constexpr int kWide = kFmt == CACHE_16 ? 1 : 2;  // (16 bits: up to eight rows, see cluster_of)
+    const auto kern = bf16 ? (wide ? attn_stream_kernel<true, kFmt, kWide, true> : attn_stream_kernel<true, kFmt, 1, true>)
+                           : (wide ? attn_stream_kernel<false, kFmt, kWide, true> : attn_stream_kernel<false, kFmt, 1, true>);
     cudaError_t e = ensure_dynamic_smem(reinterpret_cast<const void*>(kern), smem);
     if (e != cudaSuccess) return e;
     e = launch_dependent_cluster(kern, dim3(static_cast<unsigned>(p.s[0].N * p.q.Hkv * cluster)), dim3(kThreads), smem,

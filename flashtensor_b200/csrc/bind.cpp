@@ -518,6 +518,7 @@ PyObject* dequant_kv(PyObject*, PyObject* const* a, Py_ssize_t n) {
     OnDevice on({&cache.k, &cache.v, &cache.k_scale, &cache.v_scale, &idx, &len});
     if (cache.k.dim() != 4 || (idx.defined() && idx.dim() != 3)) call("asuka_b200_dequant_kv", [] { return ASUKA_ERR_BAD_SHAPE; });
     if (length < -1 || (idx.defined() && length >= 0)) call("asuka_b200_dequant_kv", [] { return ASUKA_ERR_BAD_ARGUMENT; });
+    if (length > cache.k.size(1)) call("asuka_b200_dequant_kv", [] { return ASUKA_ERR_BAD_SHAPE; });  // (before it is allocated)
     const int64_t rows = idx.defined() ? idx.size(2) : length >= 0 ? length : cache.k.size(1);
     const at::Tensor ko = empty({cache.k.size(0), rows, cache.k.size(2), cache.k.size(3)}, dtype, cache.k);
     const at::Tensor vo = empty(ko.sizes(), dtype, cache.k);

@@ -707,6 +707,7 @@ def test_refusals_on_the_device(ops):
       ("BAD_SHAPE", lambda: ops.quant_kv(q[:, :, :2], q[:, :, :2], cache, idx=torch.zeros(2, 3, 4, dtype=torch.int32, device="cuda"))),
       ("BAD_DTYPE", lambda: ops.dequant_kv(cache, torch.float32)),
       ("BAD_SHAPE", lambda: ops.dequant_kv(cache, length=65)),
+      ("BAD_SHAPE", lambda: ops.dequant_kv(cache, length=1 << 45)),  # (refused ahead of the allocation)
       ("BAD_ARGUMENT", lambda: ops.dequant_kv(cache, length=-2)),
       ("BAD_ARGUMENT", lambda: ops.dequant_kv(cache, length=3, idx=torch.zeros(2, 2, 4, dtype=torch.int32, device="cuda"))),
   ]
