@@ -15,6 +15,8 @@ from typing import Callable, List, Sequence
 
 import torch
 
+from .cache import KVCache
+
 
 class HostPipeline:
   """``submit(host_inputs, host_outputs)`` enqueues one call; ``drain()`` waits for all of them.
@@ -108,7 +110,7 @@ class GraphedCall:
   host one launch.  The graph reads the very tensors it was recorded with -- the caller refreshes
   their contents in place -- and every replay overwrites the outputs of the one before: what a
   call returns is valid until the next call with the same inputs.  Inputs are told apart by
-  address, shape, strides and dtype; at most ``max_graphs`` graphs are kept, the least recently
+  address, shape, strides and dtype (a ``KVCache`` by its tensors); at most ``max_graphs`` graphs are kept, the least recently
   used one is dropped.
 
   Replays run on the stream that is current at the call.  ``launches`` counts the kernels
@@ -121,8 +123,17 @@ class GraphedCall:
     self.launches = 0
 
   @staticmethod
-  def _key(inputs):
-    return tuple((t.data_ptr(), tuple(t.shape), t.stride(), t.dtype) for t in inputs)
+  def _tensors(inputs):
+    """The inputs, a cache's tensors in its place; None where an optional one is absent."""
+    for x in inputs:
+      if isinstance(x, KVCache):
+        yield from (x.k, x.v, x.k_scale, x.v_scale)
+      else:
+        yield x
+
+  @classmethod
+  def _key(cls, inputs):
+    return tuple(None if t is None else (t.data_ptr(), tuple(t.shape), t.stride(), t.dtype) for t in cls._tensors(inputs))
 
   def _record(self, inputs):
     from . import ops
@@ -139,7 +150,7 @@ class GraphedCall:
       outs = self.fn(*inputs)
     launches = ops.launch_count() - before
     torch.cuda.current_stream(dev).wait_stream(side)
-    return graph, outs, launches, tuple(inputs)
+    return graph, outs, launches, tuple(self._tensors(inputs))
 
   def __call__(self, *inputs):
     key = self._key(inputs)

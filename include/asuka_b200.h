@@ -220,7 +220,7 @@ int asuka_b200_dequant_kv(const asuka_dequant_kv_params* p, asuka_stream stream)
  * clamped to [0, S].  The cache and the prefix may be of different types; a 16-bit one has q's. */
 typedef struct {
   asuka_tensor q;            /* [B, Sq, H, 128] f16 | bf16; H a multiple of the cache's heads, H / Hkv <= 128 */
-  asuka_tensor out;          /* like q */
+  asuka_tensor out;          /* like q; q itself will do */
   asuka_tensor lse;          /* optional: [B, H, Sq] f32, contiguous: base-2 log-sum-exp of the scaled logits */
   asuka_kv_cache cache;      /* N = B */
   asuka_tensor len;          /* optional: [B] i32, contiguous; absent: S */

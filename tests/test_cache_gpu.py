@@ -600,6 +600,39 @@ def test_graphs_replay_with_new_contents_and_lengths(ops, fmt):
         assert same(a, b)
 
 
+def test_graphed_calls_of_the_cases_over_caches(ops):
+  # a call recorded for a cache, its scales and lengths by their addresses; an absent length is another call than a present one
+  from flashtensor_b200.host import GraphedCall
+  q, n, cache = q_of(3, 1, 8, torch.float16, 170), ints([70, 1, 33]), make_cache(3, 70, 2, torch.int8, 171)
+  prefix, wide = make_cache(1, 200, 2, torch.float16, 172), make_cache(3, 70, 2, torch.float16, 173)
+  for model, calls in ((ft().CacheAttn(2, 8), [(q, cache, n), (q, cache), (q, cache, None), (q, wide, n)]),
+                       (ft().PrefixAttn(2, 8), [(q, prefix, cache, n), (q, prefix, cache, None, ints([150])), (q, prefix, wide, n)])):
+    graphed = GraphedCall(model)
+    for _ in range(2):
+      for args in calls:
+        assert same(graphed(*args), model(*args))
+    n.copy_(ints([20, 68, 4]))
+    for args in calls:
+      assert same(graphed(*args), model(*args))
+  assert len(graphed.cache) == 3
+
+
+@pytest.mark.parametrize("fmt", [None] + FORMATS, ids=str)
+@pytest.mark.parametrize("shape", [(1, 1, 8, 2, 900, 0), (160, 1, 4, 1, 60, 0), (30, 20, 8, 4, 300, 0), (2, 90, 8, 2, 700, 0),
+                                   (40, 1, 8, 2, 50, 400), (4, 1, 8, 2, 90, 600)], ids=str)
+def test_the_output_may_take_the_place_of_q(ops, shape, fmt):
+  B, Sq, H, Hkv, cap, P = shape
+  cache = make_cache(B, cap, Hkv, fmt or torch.bfloat16, 180, torch.bfloat16)
+  q = q_of(B, Sq, H, torch.bfloat16, 181)
+  if P:
+    prefix = make_cache(1, P, Hkv, fmt or torch.bfloat16, 182, torch.bfloat16)
+    call = lambda x, out: ops.attn_prefix(x, prefix, cache, out=out)
+  else:
+    call = lambda x, out: ops.attn_cache(x, cache, out=out)
+  want, x = call(q, None), q.clone()
+  assert call(x, x).data_ptr() == x.data_ptr() and same(x, want)
+
+
 def test_no_store_lands_outside_outputs_or_workspace(ops):
   from test_parity_gpu import _Banded
   from flashtensor_b200 import _lib
