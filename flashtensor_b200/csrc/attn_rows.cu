@@ -21,8 +21,11 @@
 // the warp's 32 keys, is two f16 terms, so that a pair of codes takes two instructions.  The softmax takes the keys'
 // powers of two with the logits' factor; the values' go into the exponent, exp2(x + e - reference), and out of the row sum again.  bf16
 // queries become f16 too, a row times the power of two that puts its largest value in [1, 2).
-// (Scales as f32 in the softmax -- two multiplications and half a shared-memory read for a logit -- took it 4550 clk for a pair of
-// steps instead of 2700; half tiles of codes at a time 5300.)
+// With f16 output, finer than those roundings together (f16 keys, values and weights: 4.0e-4 to 4.8e-4 of it, the output's own 2.1e-4), and one
+// query tile the f16 tiles are the codes, exactly, and the softmax multiplies logits and weights by the scales in f32 (kExact):
+// 2.8e-4, G4 B32 H40/8 P6001 e4m3 36.9 -> 39.1 us.  bf16 output does not show them (1.7e-3 by itself), and for two query tiles, for which
+// shared memory has no room for the scales as they are, and 4550 clk a pair of steps instead of 2700 in a form that made some, it
+// stays at 3.6e-4 to 5.4e-4.  (Half tiles of codes at a time: 5300 clk.)
 #include "attn_cache.cuh"
 
 namespace asuka {
@@ -37,8 +40,10 @@ constexpr float kRescaleLimit = 6.0f;           // log2 of the largest exponenti
 
 // kPair: two query tiles; else one.  Shared memory: Q, rings of 16-bit K and V tiles; with 8 bits one ring of both in turn, one of codes,
 // and the scales that come with them.
-template <int kFmt, bool kPair> struct Cfg {
+template <bool kBF16, int kFmt, bool kPair> struct Cfg {
   static constexpr bool k8 = kFmt != CACHE_16;
+  // Scales of keys and values as f32 in the softmax, and the f16 tiles exact
+  static constexpr bool kExact = k8 && !kBF16 && !kPair;
   static constexpr int kQ = kPair ? 2 : 1;
   static constexpr int kK = k8 ? 4 : 3;                      // (8 bits: K and V in turn)
   static constexpr int kV = k8 ? 0 : (kPair ? 2 : 3);
@@ -117,13 +122,14 @@ __device__ __forceinline__ void record_timeout(uint32_t* status, uint32_t site) 
 // kFinish: one part that is all there is, and the output instead of partial results (an instantiation of its own: what a CTA does
 // once it also fetches its instructions for, and both ways in one kernel took 1.2 us longer).
 template <bool kBF16, int kFmt, bool kPair, bool kFinish>
-__global__ void __launch_bounds__(Cfg<kFmt, kPair>::kThreads, 1)
+__global__ void __launch_bounds__(Cfg<kBF16, kFmt, kPair>::kThreads, 1)
 attn_rows_kernel(const __grid_constant__ RowsMaps maps, const RowsParams p) {
-  using C = Cfg<kFmt, kPair>;
+  using C = Cfg<kBF16, kFmt, kPair>;
   extern __shared__ uint8_t smem_raw[];
   __shared__ __align__(8) Bars bars;
   // What the softmax needs of the scales of a tile's quarters: 2^e of the keys', e of the values' and 2^-e.
   __shared__ float4 powers_s[C::k8 ? C::kPowers : 1][4];
+  __shared__ float4 scales_s[C::kExact ? C::kPowers : 1][2][kTile / 4];  // (kExact) the keys', and the values' times 2^-e
   __shared__ uint8_t unit_s[C::k8 && kBF16 ? C::kQ : 1][kTile];  // exponent of a query row's power of two, as f32 has it
   __shared__ float2 row_s[kPair ? 1 : kTile];  // (one tile) second slot's reference and sum; then both slots' factors
   __shared__ uint32_t tmem_base_s;
@@ -458,7 +464,14 @@ attn_rows_kernel(const __grid_constant__ RowsMaps maps, const RowsParams p) {
           const int ke = min(max(k_top, -100), 126), ve = min(max(v_top, v_least), 126);
           v_least = max(v_least, ve - 40);
           v_up = __uint_as_float(static_cast<uint32_t>(127 - ve) << 23);
-          scale *= __uint_as_float(static_cast<uint32_t>(127 - ke) << 23);
+          if constexpr (C::kExact) {
+            float* s = reinterpret_cast<float*>(scales_s[j % C::kPowers]);
+            s[row] = scale;
+            s[kTile + row] = vs * v_up;
+            __syncwarp();
+          } else {
+            scale *= __uint_as_float(static_cast<uint32_t>(127 - ke) << 23);
+          }
           if (lane == 0) {
             powers_s[j % C::kPowers][warp - 12] = make_float4(__uint_as_float(static_cast<uint32_t>(127 + ke) << 23), static_cast<float>(ve), v_up, 0.f);
             mbar_arrive(smem_u32(&bars.powers_full[j % C::kPowers]));
@@ -487,7 +500,7 @@ attn_rows_kernel(const __grid_constant__ RowsMaps maps, const RowsParams p) {
           for (int z = 0; z < 4; ++z) {
             codes_to_f16<kFmt>(w[4 * ch + z], y[2 * z], y[2 * z + 1]);
 #pragma unroll
-            for (int x = 0; x < 2; ++x) {
+            for (int x = 0; x < (C::kExact ? 0 : 2); ++x) {
               __half2& v = *reinterpret_cast<__half2*>(&y[2 * z + x]);
               v = __hfma2(v, hi2, __hmul2(v, lo2));
             }
@@ -564,6 +577,19 @@ attn_rows_kernel(const __grid_constant__ RowsMaps maps, const RowsParams p) {
       if (C::k8 && !ok) { if (lane == 0) record_timeout(p.status, 103); break; }
       tc_fence_before_sync();
       mbar_arrive(smem_u32(&bars.s_free));
+      const float4* scale = scales_s[C::kExact ? (2 * j + t) % C::kPowers : 0][0];
+      if constexpr (C::kExact) {
+#pragma unroll
+        for (int i = 0; i < 32; ++i) {
+          const float4 f = scale[i];
+          const float2 a = __fmul2_rn(make_float2(e[4 * i], e[4 * i + 1]), make_float2(f.x, f.y));
+          const float2 b = __fmul2_rn(make_float2(e[4 * i + 2], e[4 * i + 3]), make_float2(f.z, f.w));
+          e[4 * i] = a.x;
+          e[4 * i + 1] = a.y;
+          e[4 * i + 2] = b.x;
+          e[4 * i + 3] = b.y;
+        }
+      }
       if (C::k8 && kBF16 && j == 0) mul = p.scale_log2 * __uint_as_float(static_cast<uint32_t>(unit_s[kPair ? t : 0][r_in_tile]) << 23);
       if (jk + kTile - 1 > min_lim) {
 #pragma unroll
@@ -581,7 +607,7 @@ attn_rows_kernel(const __grid_constant__ RowsMaps maps, const RowsParams p) {
       if constexpr (C::k8) {
         mx = -INFINITY;
 #pragma unroll
-        for (int g = 0; g < 4; ++g) mx = fmaxf(mx, fmaf(mx4[g], mul * power[g].x, power[g].y));
+        for (int g = 0; g < 4; ++g) mx = fmaxf(mx, fmaf(mx4[g], C::kExact ? mul : mul * power[g].x, power[g].y));
       } else {
         mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * mul;
       }
@@ -619,7 +645,7 @@ attn_rows_kernel(const __grid_constant__ RowsMaps maps, const RowsParams p) {
       if constexpr (C::k8) {
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
-          const float f = mul * power[g].x, up = power[g].y - ref;
+          const float f = C::kExact ? mul : mul * power[g].x, up = power[g].y - ref;
           const float2 mul2 = make_float2(f, f), up2 = make_float2(up, up);
 #pragma unroll
           for (int i = 16 * g; i < 16 * g + 16; ++i) {
@@ -627,6 +653,7 @@ attn_rows_kernel(const __grid_constant__ RowsMaps maps, const RowsParams p) {
             v.x = ex2(v.x);
             v.y = ex2(v.y);
             ts4[g] = __fadd2_rn(ts4[g], v);
+            if constexpr (C::kExact) v = __fmul2_rn(v, reinterpret_cast<const float2*>(scale + kTile / 4)[i]);
             pk[i] = pack2<false>(v.x, v.y);
           }
           l = fmaf(ts4[g].x + ts4[g].y, power[g].z, l);
@@ -936,7 +963,7 @@ Tiles tiles_of(const Segment& s, const RowShape& q) {
 
 template <bool kBF16, int kFmt, bool kPair, bool kFinish>
 cudaError_t launch_rows_of(const CacheRows& c, const CacheAttnArgs& a, RowsParams& p, const Tiles& tiles, cudaStream_t stream) {
-  using C = Cfg<kFmt, kPair>;
+  using C = Cfg<kBF16, kFmt, kPair>;
   RowsMaps maps;
   const uint32_t box[4] = {64, static_cast<uint32_t>(p.q.group), static_cast<uint32_t>(tiles.pos), static_cast<uint32_t>(tiles.b)};
   if (tma_host::make_boxed_map(&maps.q, a.q, kBF16, a.B, a.Sq, a.H, 128, a.q_sb, a.q_ss, a.q_sh, box) ||
