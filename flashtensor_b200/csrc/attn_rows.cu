@@ -1057,7 +1057,8 @@ cudaError_t launch_attn_merge(const CacheAttnArgs& a, const Source& first, const
   p.o_sb = a.o_sb; p.o_ss = a.o_ss; p.o_sh = a.o_sh;
   p.lse2 = a.lse2;
   p.B = a.B;
-  // Parts of a row: as many as it is given, or as workers share a unit.  A warp has eight in flight.
+  // Parts of a row: as many as it is given, or as workers share a unit.  A warp has kBatch in flight; eight warps to a row from 17 on
+  // (from 11 on, 128 sequences behind 32768 bf16 rows took 23 us longer).
   int64_t parts = 0;
   for (const Source* f : {&first, &second}) {
     if (f->dealt) {
