@@ -411,7 +411,7 @@ attn_rows_kernel(const __grid_constant__ RowsMaps maps, const RowsParams p) {
               top = max3(top, fabsf(v.x), fabsf(v.y));
             }
           }
-          // (rows of zeros, and of nothing but values under 2^-100, stay as they are or vanish)
+          // (rows of zeros, and of nothing but values under 2^-100, stay as they are or vanish: logits of 0)
           const int e = min(max(static_cast<int>(__float_as_uint(top) >> 23), 27), 253);
           const float down = __uint_as_float(static_cast<uint32_t>(254 - e) << 23);
           unit_s[t][row] = static_cast<uint8_t>(e);
@@ -604,10 +604,14 @@ attn_rows_kernel(const __grid_constant__ RowsMaps maps, const RowsParams p) {
         for (int g = 0; g < 4; ++g) mx4[g] = max3(mx4[g], e[32 * g + i], e[32 * g + i + 1]);
       }
       float mx;
+      [[maybe_unused]] float factor[4];  // (8 bits) of the quarters' logits; not 0, which masked ones, -inf, would make NaN
       if constexpr (C::k8) {
         mx = -INFINITY;
 #pragma unroll
-        for (int g = 0; g < 4; ++g) mx = fmaxf(mx, fmaf(mx4[g], C::kExact ? mul : mul * power[g].x, power[g].y));
+        for (int g = 0; g < 4; ++g) {
+          factor[g] = C::kExact ? mul : fmaxf(mul * power[g].x, 0x1p-126f);
+          mx = fmaxf(mx, fmaf(mx4[g], factor[g], power[g].y));
+        }
       } else {
         mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * mul;
       }
@@ -645,8 +649,8 @@ attn_rows_kernel(const __grid_constant__ RowsMaps maps, const RowsParams p) {
       if constexpr (C::k8) {
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
-          const float f = C::kExact ? mul : mul * power[g].x, up = power[g].y - ref;
-          const float2 mul2 = make_float2(f, f), up2 = make_float2(up, up);
+          const float up = power[g].y - ref;
+          const float2 mul2 = make_float2(factor[g], factor[g]), up2 = make_float2(up, up);
 #pragma unroll
           for (int i = 16 * g; i < 16 * g + 16; ++i) {
             float2 v = __ffma2_rn(make_float2(e[2 * i], e[2 * i + 1]), mul2, up2);

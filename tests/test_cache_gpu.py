@@ -755,3 +755,32 @@ def test_refusals_on_the_device(ops):
     ft().CacheAttn(4, 4).forward(q, cache)
   with pytest.raises(TypeError):
     ops.dequant_kv(cache, "bfloat16")
+
+
+# ------------------------------------------------------------------------------------------
+# the ends of the range
+# ------------------------------------------------------------------------------------------
+# streamed (a cluster to a unit, dealt out), one query tile of many rows, two: B, Sq, group
+FORMS = [(1, 1, 4), (50, 1, 4), (2, 20, 2), (2, 100, 2)]
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("fmt", [None] + FORMATS, ids=str)
+@pytest.mark.parametrize("n", [1, 129, 296, 352, 384])
+@pytest.mark.parametrize("B, Sq, group", FORMS)
+def test_query_rows_of_zeros_and_tiny_ones(ops, B, Sq, group, n, fmt, dtype):
+  # logits of 0 or nearly: the mean of what the row sees, whatever lies behind the sequence or the mask (there are keys of zeros too)
+  cache = make_cache(B, 400, 2, fmt or dtype, 190, dtype)
+  cache.k[:, 300:] = 0
+  if fmt is not None:
+    cache.k_scale[:, :, 300:] = 2.0 ** -100
+  q = q_of(B, Sq, 2 * group, dtype, 191)
+  q[0] = 0
+  q[-1, :, ::2] *= 0 if dtype == torch.float16 else 2.0 ** -90
+  q[-1, Sq // 2:, 1::2] *= 2.0 ** -20
+  prefix = make_cache(1, 330, 2, fmt or dtype, 192, dtype)
+  lens = [n] * B
+  for causal in (True, False):
+    check_attention(*ops.attn_cache(q, cache, ints(lens), causal=causal, return_lse=True), _attention(q, cache, lens, causal), f"causal={causal}")
+    check_attention(*ops.attn_prefix(q, prefix, cache, ints(lens), causal=causal, return_lse=True),
+                    _attention(q, cache, lens, causal, prefix), f"prefix, causal={causal}")
