@@ -694,10 +694,17 @@ int check_scale(asuka_tensor* t, const asuka_tensor& rows) {
   return ASUKA_OK;
 }
 
+// A tensor of no elements has no address either, but is not an absent one.
+bool is_empty(const asuka_tensor& t) {
+  for (int i = 0; i < t.ndim && i < 5; ++i)
+    if (t.shape[i] == 0) return true;
+  return false;
+}
+
 // optional [n] i32
 int check_counts(const asuka_tensor& t, int64_t n, const int32_t** out) {
   *out = nullptr;
-  if (t.ptr == nullptr) return ASUKA_OK;
+  if (t.ptr == nullptr) return is_empty(t) ? ASUKA_ERR_BAD_SHAPE : ASUKA_OK;
   if (t.dtype != ASUKA_I32) return ASUKA_ERR_BAD_DTYPE;
   if (t.ndim != 1 || t.shape[0] != n) return ASUKA_ERR_BAD_SHAPE;
   if (n != 1 && t.stride[0] != 1) return ASUKA_ERR_BAD_STRIDE;
@@ -709,7 +716,7 @@ int check_counts(const asuka_tensor& t, int64_t n, const int32_t** out) {
 // optional [B, H, n] i32
 int check_idx(const asuka_tensor& t, int64_t B, int64_t H, const int32_t** out, int64_t* n) {
   *out = nullptr;
-  if (t.ptr == nullptr) return ASUKA_OK;
+  if (t.ptr == nullptr) return is_empty(t) ? ASUKA_ERR_BAD_SHAPE : ASUKA_OK;
   if (t.ndim != 3 || t.shape[2] <= 0) return ASUKA_ERR_BAD_SHAPE;
   if (t.shape[2] > (1 << 24)) return ASUKA_ERR_TOO_LARGE;
   const int64_t shape[3] = {B, H, t.shape[2]};

@@ -194,7 +194,7 @@ typedef struct {
  * Rows from count[b] on (padding) and rows that would land outside [0, S) are not written. */
 typedef struct {
   asuka_tensor k, v;    /* [B, T, Hkv, 128] f16 | bf16, same type, strides as for asuka_b200_attn_fwd */
-  asuka_tensor idx;     /* optional: [B, Hkv, n] i32, contiguous (n rows are written instead of T) */
+  asuka_tensor idx;     /* optional: [B, Hkv, n] i32, n >= 1, contiguous (n rows are written instead of T) */
   asuka_tensor start;   /* optional: [B] i32, contiguous; absent: 0 */
   asuka_tensor count;   /* optional: [B] i32, contiguous; absent: all rows */
   asuka_kv_cache cache; /* N = B; must not overlap k and v */

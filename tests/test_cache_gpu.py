@@ -784,3 +784,19 @@ def test_query_rows_of_zeros_and_tiny_ones(ops, B, Sq, group, n, fmt, dtype):
     check_attention(*ops.attn_cache(q, cache, ints(lens), causal=causal, return_lse=True), _attention(q, cache, lens, causal), f"causal={causal}")
     check_attention(*ops.attn_prefix(q, prefix, cache, ints(lens), causal=causal, return_lse=True),
                     _attention(q, cache, lens, causal, prefix), f"prefix, causal={causal}")
+
+
+def test_empty_indices_lengths_and_counts_are_refused(ops):
+  # a tensor of no elements has no address, which is how an absent one is told: a selection of nothing would write every row
+  from flashtensor_b200 import _lib
+  cache = ft().KVCache.empty(2, 64, 2)
+  for t in (cache.k, cache.v):
+    t.view(torch.uint8).fill_(0x5a)
+  q, new = (torch.ones(2, 3, h, D, dtype=torch.float16, device="cuda") for h in (4, 2))
+  none, no_idx = ints([]), torch.empty(2, 2, 0, dtype=torch.int32, device="cuda")
+  for call in (lambda: cache.write(new, new, idx=no_idx), lambda: cache.write(new, new, start=none), lambda: cache.write(new, new, count=none),
+               lambda: cache.read(torch.float16, idx=no_idx), lambda: cache.read(torch.float16, kv_len=none), lambda: ops.attn_cache(q, cache, none),
+               lambda: ops.attn_prefix(q, cache, cache, None, none), lambda: ops.attn_prefix(q, cache, cache, none)):
+    with pytest.raises(_lib.AsukaError):
+      call()
+  assert (cache.k.contiguous().view(torch.uint8) == 0x5a).all() and (cache.v.contiguous().view(torch.uint8) == 0x5a).all()

@@ -110,6 +110,19 @@ def test_write_and_read_refuse(built_lib):
   assert get(len=_t((3,), dtype=I32)) == -3
 
 
+def test_a_tensor_of_no_elements_is_not_an_absent_one(built_lib):
+  # (it has no address either)
+  lib = _lib.load()
+  x, no, none, no_idx = _t((2, 5, 2, 128)), _lib.Tensor(), _t((0,), dtype=I32, ptr=0), _t((2, 2, 0), dtype=I32, ptr=0)
+  for idx, start, count in ((no_idx, no, no), (no, none, no), (no, no, none)):
+    assert lib.asuka_b200_quant_kv(ctypes.byref(_lib.QuantKvParams(x, x, idx, start, count, _cache())), None) == -3
+  out = _t((2, 64, 2, 128))
+  for idx, n in ((no_idx, no), (no, none)):
+    assert lib.asuka_b200_dequant_kv(ctypes.byref(_lib.DequantKvParams(_cache(), idx, n, out, out)), None) == -3
+  assert _attn(lib, len=none) == -3
+  assert _attn(lib, prefix=_cache(N=1), plen=none) == -3
+
+
 def test_operators_refuse_tensors_on_the_host(built_lib):
   from flashtensor_b200 import ops
   cache = ft.KVCache.empty(1, 8, 2, device="cpu")
