@@ -137,7 +137,7 @@ class GraphedCall:
 
   def _record(self, inputs):
     from . import ops
-    dev = inputs[0].device
+    dev = next(t for t in self._tensors(inputs) if t is not None).device
     side = torch.cuda.Stream(device=dev)
     side.wait_stream(torch.cuda.current_stream(dev))
     with torch.cuda.stream(side):

@@ -800,3 +800,24 @@ def test_empty_indices_lengths_and_counts_are_refused(ops):
     with pytest.raises(_lib.AsukaError):
       call()
   assert (cache.k.contiguous().view(torch.uint8) == 0x5a).all() and (cache.v.contiguous().view(torch.uint8) == 0x5a).all()
+
+
+def test_graphed_calls_whose_first_input_is_a_cache_or_absent(ops):
+  from flashtensor_b200.host import GraphedCall
+  cache, q, n = make_cache(2, 60, 2, torch.int8, 200), q_of(2, 1, 8, torch.float16, 201), ints([60, 7])
+  attend = GraphedCall(lambda c, x, m: ops.attn_cache(x, c, m))
+  last = GraphedCall(lambda m, x, c: ops.attn_cache(x, c, m))
+  for _ in range(2):
+    assert same(attend(cache, q, n), ops.attn_cache(q, cache, n))
+    assert same(last(None, q, cache), ops.attn_cache(q, cache))
+  # a write, whose rows and place change between replays
+  k, v = (torch.zeros(2, 1, 2, D, dtype=torch.float16, device="cuda") for _ in range(2))
+  write = GraphedCall(lambda c, *rest: c.write(*rest).k)
+  plain = ft().KVCache(*[t.clone(memory_format=torch.preserve_format) for t in (cache.k, cache.v, cache.k_scale, cache.v_scale)])
+  for t in range(3):
+    for x, seed in ((k, 202), (v, 203)):
+      x.copy_(torch.randn(x.shape, generator=gen(seed + 10 * t), device="cuda"))
+    n.copy_(ints([3 * t, 50 + t]))
+    write(cache, k, v, n)
+    plain.write(k, v, start=n)
+    assert same(cache.k, plain.k) and same(cache.v, plain.v) and torch.equal(cache.v_scale, plain.v_scale)
