@@ -20,6 +20,25 @@ __device__ __forceinline__ float lg2(float x) {
   asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+// Over 8 bits the reference of a row's exponentials contains the values' scales (2^-76 to 2^121, smaller ones count as 2^-76), so that
+// the largest term of their sum may be anything from 2^-121 to 2^76, and one that counts a little less.  While they are summed
+// they are kept times 2^kLift: neither end leaves f32's normal numbers, and what a term may lose is below 2^-28 of the largest.
+// What takes a sum from one reference to the next may be smaller than any of those; it comes as the square of `half_step`.
+constexpr int kLeast = -76;
+constexpr float kLeastScale = 0x1p-76f;
+constexpr int kLift = 24;
+constexpr float kLiftUp = 0x1p24f, kLiftDown = 0x1p-24f;
+__device__ __forceinline__ float half_step(float from, float to) { return ex2(0.5f * (from - to)); }
+// (Without scales above kLarge a sum is 2^-20 at least, and no reference that counts is 2^126 below another's.)
+constexpr float kLarge = 0x1p20f;
+// Such a sum and its reference as others are: the sum in [0.5, 1), the reference with what that takes.  Returns what takes the
+// weighted values along.  (Nothing seen, or nothing but NaN, stays what it is.)
+__device__ __forceinline__ float unlift(float& ref, float& sum) {
+  const int e = min(max(static_cast<int>(__float_as_uint(sum) >> 23 & 0xffu), 25), 252) - 126;  // (both factors normal numbers)
+  sum *= __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
+  ref += static_cast<float>(e - kLift);
+  return __uint_as_float(static_cast<uint32_t>(127 + kLift - e) << 23);
+}
 template <bool kBF16>
 __device__ __forceinline__ float2 unpack2(uint32_t w) {
   if constexpr (kBF16) return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&w));

@@ -18,7 +18,7 @@
 // the stage is free again, and writes them times their scale in the two swizzled halves that the tensor pipe reads, neither with a
 // bank conflict; where the next tile has landed, its codes are loaded between the stores (G4 B32 H40/8 P6001 e4m3 37.9 -> 36.9 us, two query
 // tiles unchanged).  A code times its scale is rounded once, to f16 (2^-12 on average): the scale, under the power of two of the largest of
-// the warp's 32 keys, is two f16 terms, so that a pair of codes takes two instructions.  The softmax takes the keys'
+// the warp's 32 keys or of the tile's 128 values, is two f16 terms, so that a pair of codes takes two instructions.  The softmax takes the keys'
 // powers of two with the logits' factor; the values' go into the exponent, exp2(x + e - reference), and out of the row sum again.  bf16
 // queries become f16 too, a row times the power of two that puts its largest value in [1, 2).
 // With f16 output, finer than those roundings together (f16 keys, values and weights: 4.0e-4 to 4.8e-4 of it, the output's own 2.1e-4), and one
@@ -127,11 +127,13 @@ attn_rows_kernel(const __grid_constant__ RowsMaps maps, const RowsParams p) {
   using C = Cfg<kBF16, kFmt, kPair>;
   extern __shared__ uint8_t smem_raw[];
   __shared__ __align__(8) Bars bars;
-  // What the softmax needs of the scales of a tile's quarters: 2^e of the keys', e of the values' and 2^-e.
-  __shared__ float4 powers_s[C::k8 ? C::kPowers : 1][4];
+  // What the softmax needs of the scales of a tile: 2^e of the keys' for each quarter, e of the values' and 2^(kLift - e).
+  __shared__ float4 k_power_s[C::k8 && !C::kExact ? C::kPowers : 1];
+  __shared__ float2 v_power_s[C::k8 ? C::kPowers : 1];
   __shared__ float4 scales_s[C::kExact ? C::kPowers : 1][2][kTile / 4];  // (kExact) the keys', and the values' times 2^-e
   __shared__ uint8_t unit_s[C::k8 && kBF16 ? C::kQ : 1][kTile];  // exponent of a query row's power of two, as f32 has it
   __shared__ float2 row_s[kPair ? 1 : kTile];  // (one tile) second slot's reference and sum; then both slots' factors
+  __shared__ float take_s[C::k8 && !kPair ? kTile : 1];  // (one tile) second slot's `take`
   __shared__ uint32_t tmem_base_s;
   __shared__ uint32_t abort_s;
 
@@ -433,8 +435,8 @@ attn_rows_kernel(const __grid_constant__ RowsMaps maps, const RowsParams p) {
       }
       const int row = tid - 384;
       float vs = 0.f;               // the row's value scale, from the keys' turn to the values'
-      float v_up = 0.f;             // 2^-e of the warp's 32
-      int v_least = -80;            // (e does not fall by more than 40 from its largest, nor so low that a row sum could suffer)
+      float v_up = 0.f;             // 2^-e of the tile
+      int v_least = kLeast;         // (e does not fall by more than 40 from its largest: what is smaller still is lost in an output)
       uint32_t w[32];               // the row's codes
       bool loaded = false;          // (under the conversion of the tile before)
       for (int c = 0; c < 2 * n && ok; ++c) {
@@ -451,18 +453,31 @@ attn_rows_kernel(const __grid_constant__ RowsMaps maps, const RowsParams p) {
         }
         float scale;
         if (!is_v) {
-          const uint32_t at = sRawScale + st % C::kRawScales * 1024 + row * 4;
-          scale = live ? ldsf(at) : 0.f;
-          vs = live ? ldsf(at + 512) : 0.f;
-          // exponents of the largest of the warp's 32 keys (of what is finite: the others are what they are)
+          const uint32_t at = sRawScale + st % C::kRawScales * 1024;
+          scale = live ? ldsf(at + row * 4) : 0.f;
+          vs = live ? ldsf(at + 512 + row * 4) : 0.f;
+          // exponents of the largest of the warp's 32 key scales, and of all 128 value scales: the four warps' are the same, so that
+          // none falls far below the others' in the softmax (of what is finite: the others are what they are)
           auto bits = [](float x) {
             const uint32_t b = __float_as_uint(x) & 0x7fffffffu;
             return b < 0x7f800000u ? b : 0u;
           };
-          const int k_top = static_cast<int>(__reduce_max_sync(0xffffffffu, bits(scale)) >> 23) - 127;
-          const int v_top = static_cast<int>(__reduce_max_sync(0xffffffffu, bits(vs)) >> 23) - 127;
-          const int ke = min(max(k_top, -100), 126), ve = min(max(v_top, v_least), 126);
-          v_least = max(v_least, ve - 40);
+          auto exponent = [](uint32_t b) { return static_cast<int>(__reduce_max_sync(0xffffffffu, b) >> 23) - 127; };
+          [[maybe_unused]] int ke;
+          if constexpr (!C::kExact) {
+            ke = min(max(exponent(bits(scale)), -100), 126);
+          }
+          float four[4];
+          lds4(at + 512 + lane * 16, reinterpret_cast<uint32_t*>(four));
+          const int there = len - (j0 + j) * kTile;  // (what lies behind the sequence may be anything)
+          if (there < kTile) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) four[i] = lane * 4 + i < there ? four[i] : 0.f;
+          }
+          int v_top = exponent(__float_as_uint(fmaxf(fmaxf(fabsf(four[0]), fabsf(four[1])), fmaxf(fabsf(four[2]), fabsf(four[3])))));
+          if (v_top == 128) v_top = exponent(max(max(bits(four[0]), bits(four[1])), max(bits(four[2]), bits(four[3]))));
+          v_least = max(v_least, v_top - 40);
+          const int ve = min(max(v_top, v_least), 126);
           v_up = __uint_as_float(static_cast<uint32_t>(127 - ve) << 23);
           if constexpr (C::kExact) {
             float* s = reinterpret_cast<float*>(scales_s[j % C::kPowers]);
@@ -473,7 +488,9 @@ attn_rows_kernel(const __grid_constant__ RowsMaps maps, const RowsParams p) {
             scale *= __uint_as_float(static_cast<uint32_t>(127 - ke) << 23);
           }
           if (lane == 0) {
-            powers_s[j % C::kPowers][warp - 12] = make_float4(__uint_as_float(static_cast<uint32_t>(127 + ke) << 23), static_cast<float>(ve), v_up, 0.f);
+            if constexpr (!C::kExact)
+              reinterpret_cast<float*>(&k_power_s[j % C::kPowers])[warp - 12] = __uint_as_float(static_cast<uint32_t>(127 + ke) << 23);
+            if (warp == 12) v_power_s[j % C::kPowers] = make_float2(static_cast<float>(ve), v_up * kLiftUp);
             mbar_arrive(smem_u32(&bars.powers_full[j % C::kPowers]));
           }
         } else {
@@ -550,7 +567,7 @@ attn_rows_kernel(const __grid_constant__ RowsMaps maps, const RowsParams p) {
     }
     bool ok = true;
     float m_ref = -INFINITY;             // exponent reference of this row, in log2 units of the scaled logit
-    float l = 0.f;                       // row sum under the current reference
+    float l = 0.f;                       // row sum under the current reference; 8 bits: times 2^kLift
     for (int j = 0; j < n_t && ok; ++j) {
       ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&bars.s_full[t]), j & 1, abortp));
       if (!ok) { if (lane == 0) record_timeout(p.status, 100); break; }
@@ -559,7 +576,8 @@ attn_rows_kernel(const __grid_constant__ RowsMaps maps, const RowsParams p) {
       const int thr = lim - jk;  // columns > thr of this tile are masked for this row
       // The whole 128-wide row goes to registers at once, and S to the next QK^T.
       float e[128];
-      float4 power[4];  // (8 bits) of the tile's quarters
+      float4 k_power;   // (8 bits) of the tile's quarters
+      float2 v_power;
       {
         uint32_t(&u)[128] = *reinterpret_cast<uint32_t(*)[128]>(e);
         tmem_ld32(tS + 0, *reinterpret_cast<uint32_t(*)[32]>(&u[0]));
@@ -569,8 +587,8 @@ attn_rows_kernel(const __grid_constant__ RowsMaps maps, const RowsParams p) {
         if constexpr (C::k8) {
           const int c = kPair ? j : 2 * j + t;  // the tile, of the CTA's
           ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&bars.powers_full[c % C::kPowers]), (c / C::kPowers) & 1, abortp));
-#pragma unroll
-          for (int g = 0; g < 4; ++g) power[g] = powers_s[c % C::kPowers][g];
+          if constexpr (!C::kExact) k_power = k_power_s[c % C::kPowers];
+          v_power = v_power_s[c % C::kPowers];
         }
         tmem_wait_ld();
       }
@@ -606,11 +624,17 @@ attn_rows_kernel(const __grid_constant__ RowsMaps maps, const RowsParams p) {
       float mx;
       [[maybe_unused]] float factor[4];  // (8 bits) of the quarters' logits; not 0, which masked ones, -inf, would make NaN
       if constexpr (C::k8) {
-        mx = -INFINITY;
+        if constexpr (C::kExact) {
+          mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * mul + v_power.x;
+        } else {
+          const float of[4] = {k_power.x, k_power.y, k_power.z, k_power.w};
+          mx = -INFINITY;
 #pragma unroll
-        for (int g = 0; g < 4; ++g) {
-          factor[g] = C::kExact ? mul : fmaxf(mul * power[g].x, 0x1p-126f);
-          mx = fmaxf(mx, fmaf(mx4[g], factor[g], power[g].y));
+          for (int g = 0; g < 4; ++g) {
+            factor[g] = fmaxf(mul * of[g], 0x1p-126f);
+            mx = fmaxf(mx, mx4[g] * factor[g]);
+          }
+          mx += v_power.x;
         }
       } else {
         mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * mul;
@@ -622,9 +646,10 @@ attn_rows_kernel(const __grid_constant__ RowsMaps maps, const RowsParams p) {
         if (__any_sync(0xffffffffu, need)) {
           float alpha = 1.f;
           if (need) {
-            alpha = ex2(m_ref - mx);
+            const float step = C::k8 ? half_step(m_ref, mx) : ex2(m_ref - mx);
+            alpha = C::k8 ? step * step : step;
             m_ref = mx;
-            l *= alpha;
+            l = (C::k8 ? l * step : l) * step;
           }
           // O_t is the sum over this slot's earlier tiles, complete with their last P.V
           ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&bars.pv_done[t]), (j - 1) & 1, abortp));
@@ -647,10 +672,12 @@ attn_rows_kernel(const __grid_constant__ RowsMaps maps, const RowsParams p) {
       float2 ts4[4] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f), make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
       uint32_t pk[64];
       if constexpr (C::k8) {
+        const float up = v_power.x - ref;
+        const float2 up2 = make_float2(up, up);
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
-          const float up = power[g].y - ref;
-          const float2 mul2 = make_float2(factor[g], factor[g]), up2 = make_float2(up, up);
+          const float f = C::kExact ? mul : factor[g];
+          const float2 mul2 = make_float2(f, f);
 #pragma unroll
           for (int i = 16 * g; i < 16 * g + 16; ++i) {
             float2 v = __ffma2_rn(make_float2(e[2 * i], e[2 * i + 1]), mul2, up2);
@@ -660,7 +687,7 @@ attn_rows_kernel(const __grid_constant__ RowsMaps maps, const RowsParams p) {
             if constexpr (C::kExact) v = __fmul2_rn(v, reinterpret_cast<const float2*>(scale + kTile / 4)[i]);
             pk[i] = pack2<false>(v.x, v.y);
           }
-          l = fmaf(ts4[g].x + ts4[g].y, power[g].z, l);
+          l = fmaf(ts4[g].x + ts4[g].y, v_power.y, l);
         }
       } else {
         const float2 mul2 = make_float2(mul, mul), neg_m2 = make_float2(-ref, -ref);
@@ -692,6 +719,7 @@ attn_rows_kernel(const __grid_constant__ RowsMaps maps, const RowsParams p) {
       tc_fence_after_sync();
     }
     // ---- the part's results: unnormalised O, reference, sum
+    const float take = C::k8 ? unlift(m_ref, l) : 1.f;  // (of this slot's O)
     if (l == 0.f) m_ref = -INFINITY;                // (nothing seen)
     else if (!(m_ref > -INFINITY)) m_ref = 0.f;     // (nothing but NaN: the sum)
     if constexpr (!kFinish) {
@@ -705,6 +733,10 @@ attn_rows_kernel(const __grid_constant__ RowsMaps maps, const RowsParams p) {
             uint32_t o[32];
             tmem_ld32(tO + c * 32, o);
             tmem_wait_ld();
+            if constexpr (C::k8) {
+#pragma unroll
+              for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * take);
+            }
             if (live) {
 #pragma unroll
               for (int g = 0; g < 4; ++g) st_global_v8(orow + c * 32 + g * 8, &o[g * 8]);
@@ -714,7 +746,10 @@ attn_rows_kernel(const __grid_constant__ RowsMaps maps, const RowsParams p) {
       } else {
         // the slots' factors to a common reference; each writes half of the columns
         // (every softmax warp gets to the barriers, expired waits or not)
-        if (t == 1) row_s[r_in_tile] = make_float2(m_ref, l);
+        if (t == 1) {
+          row_s[r_in_tile] = make_float2(m_ref, l);
+          if constexpr (C::k8) take_s[r_in_tile] = take;
+        }
         tc_fence_before_sync();
         named_bar_sync(1, 256);
         float f0, f1;
@@ -723,8 +758,12 @@ attn_rows_kernel(const __grid_constant__ RowsMaps maps, const RowsParams p) {
           const float mm = fmaxf(m_ref, o.x);
           f0 = m_ref > -INFINITY ? ex2(m_ref - mm) : 0.f;
           f1 = o.x > -INFINITY ? ex2(o.x - mm) : 0.f;
-          row_s[r_in_tile] = make_float2(f0, f1);
           if (live) *ml = make_float2(mm, fmaf(f1, o.y, f0 * l));
+          if constexpr (C::k8) {
+            f0 *= take;
+            f1 *= take_s[r_in_tile];
+          }
+          row_s[r_in_tile] = make_float2(f0, f1);
         }
         named_bar_sync(1, 256);
         tc_fence_after_sync();
@@ -764,9 +803,12 @@ attn_rows_kernel(const __grid_constant__ RowsMaps maps, const RowsParams p) {
         for (int i = 0; i < 4; ++i)
           *reinterpret_cast<uint4*>(p.out + out_at + col + 8 * i) = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
       };
-      float f0 = l == 0.f ? 0.f : 1.f / l, f1 = 0.f, ref = m_ref, sum = l;
+      float f0 = l == 0.f ? 0.f : take / l, f1 = 0.f, ref = m_ref, sum = l;
       if constexpr (!kPair) {
-        if (t == 1) row_s[r_in_tile] = make_float2(m_ref, l);
+        if (t == 1) {
+          row_s[r_in_tile] = make_float2(m_ref, l);
+          if constexpr (C::k8) take_s[r_in_tile] = take;
+        }
         tc_fence_before_sync();
         named_bar_sync(1, 256);
         if (t == 0) {
@@ -776,8 +818,8 @@ attn_rows_kernel(const __grid_constant__ RowsMaps maps, const RowsParams p) {
           f1 = o.x > -INFINITY ? ex2(o.x - ref) : 0.f;
           sum = fmaf(f1, o.y, f0 * l);
           const float inv = sum == 0.f ? 0.f : 1.f / sum;
-          f0 *= inv;
-          f1 *= inv;
+          f0 *= inv * take;
+          f1 *= C::k8 ? inv * take_s[r_in_tile] : inv;
           row_s[r_in_tile] = make_float2(f0, f1);
         }
         named_bar_sync(1, 256);

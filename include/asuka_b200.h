@@ -217,7 +217,9 @@ int asuka_b200_dequant_kv(const asuka_dequant_kv_params* p, asuka_stream stream)
  *   - the prefix (optional) holds G sequences, each shared by B / G consecutive sequences of q, which
  *     see all of its first prefix_len[g] rows.
  * One softmax goes over both; a row that sees nothing is 0 with the log-sum-exp -inf.  Lengths are
- * clamped to [0, S].  The cache and the prefix may be of different types; a 16-bit one has q's. */
+ * clamped to [0, S].  The cache and the prefix may be of different types; a 16-bit one has q's.
+ * Values of 8 bits are weighted in f16 under a power of two of the largest ones (and of no less than the scale
+ * 2^-76: values far below that lose bits). */
 typedef struct {
   asuka_tensor q;            /* [B, Sq, H, 128] f16 | bf16; H a multiple of the cache's heads, H / Hkv <= 128 */
   asuka_tensor out;          /* like q; q itself will do */

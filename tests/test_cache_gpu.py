@@ -821,3 +821,38 @@ def test_graphed_calls_whose_first_input_is_a_cache_or_absent(ops):
     write(cache, k, v, n)
     plain.write(k, v, start=n)
     assert same(cache.k, plain.k) and same(cache.v, plain.v) and torch.equal(cache.v_scale, plain.v_scale)
+
+
+# 2^125: values up to 2^127 of bf16's largest 2^128, scales 2^120; 2^-60: scales down to 2^-69
+@pytest.mark.parametrize("fmt", FORMATS, ids=str)
+@pytest.mark.parametrize("order", ["large", "small", "large first", "small first", "mixed", "mixed by 32", "zeros"])
+@pytest.mark.parametrize("B, Sq, group", [*FORMS, (3, 4, 4)])
+def test_values_at_the_ends_of_the_range(ops, B, Sq, group, order, fmt):
+  # what the weights' sum holds may not depend on the size of the values, which is in the exponentials' reference
+  S, P = 1100, 700
+  def sized(c):
+    n = c.k.shape[1]
+    size = torch.full(c.v_scale.shape, 2.0 ** 125, device="cuda")
+    j, g = torch.arange(n, device="cuda"), gen(210)
+    if order == "small":
+      size[:] = 2.0 ** -60
+    elif order == "large first":
+      size[..., 400:] = 1.0
+    elif order == "small first":
+      size[..., :400] = 2.0 ** -60
+    elif order == "mixed":
+      size = torch.exp2(125.0 * torch.randint(0, 2, size.shape, generator=g, device="cuda"))
+    elif order == "mixed by 32":
+      size = torch.exp2(torch.tensor([125.0, 0.0, -60.0], device="cuda")[(j // 32) % 3]).expand_as(size)
+    elif order == "zeros":  # (rows of zeros have the smallest scale there is)
+      size[..., 100:] = 1e30
+      c.v.view(torch.uint8)[:, 200:] = 0
+      c.v_scale[..., 200:], size[..., 200:] = 2.0 ** -100, 1.0
+    c.v_scale *= size
+    return c
+  prefix, cache = sized(make_cache(1, P, 2, fmt, 211, torch.bfloat16)), sized(make_cache(B, S, 2, fmt, 212, torch.bfloat16))
+  q, lens = q_of(B, Sq, 2 * group, torch.bfloat16, 213, 2.0), [S - 31 * i % 500 for i in range(B)]
+  check_attention(*ops.attn_cache(q, cache, ints(lens), return_lse=True), _attention(q, cache, lens))
+  check_attention(*ops.attn_prefix(q, prefix, cache, ints(lens), return_lse=True), _attention(q, cache, lens, True, prefix), "prefix")
+  plain = make_cache(1, P, 2, torch.bfloat16, 214, torch.bfloat16)  # (values of ordinary size, without scales, ahead of them)
+  check_attention(*ops.attn_prefix(q, plain, cache, ints(lens), return_lse=True), _attention(q, cache, lens, True, plain), "16-bit prefix")
