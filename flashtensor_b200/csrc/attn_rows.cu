@@ -189,12 +189,14 @@ attn_rows_kernel(const __grid_constant__ RowsMaps maps, const RowsParams p) {
   if (!p.chained) griddep_wait();
   griddep_launch_dependents();
 
-  // This CTA's key tiles: its part of what the sequence has, and of what the block's last rows see.
+  // This CTA's key tiles: its part of what the sequence has, and of what the block's last rows see.  (A causal segment is of the
+  // sequences' own rows: a block's tiles are of one sequence, next to each other.  A prompt of 1000, 2000, 4000 tokens, 32 heads over 8,
+  // 16 bits: 20.6, 53.8, 245 us, to the end of the sequence for every block of two tiles 22.8, 68.7, 333.)
   const int len = seen_of(p.s, seq);
   int limit = len;
   if (p.s.causal) {
     const int last = min(tile0 + (two ? 1 : 0), p.tiles - 1) % p.pos_tiles;
-    const int last_pos = p.pos_tiles == 1 || two ? p.q.Sq - 1 : min((last + 1) * p.tile_pos, p.q.Sq) - 1;
+    const int last_pos = p.pos_tiles == 1 ? p.q.Sq - 1 : min((last + 1) * p.tile_pos, p.q.Sq) - 1;
     limit = max(0, min(len, last_pos + len - p.q.Sq + 1));
   }
   const int all = (limit + kTile - 1) / kTile;

@@ -218,6 +218,8 @@ int asuka_b200_dequant_kv(const asuka_dequant_kv_params* p, asuka_stream stream)
  *     see all of its first prefix_len[g] rows.
  * One softmax goes over both; a row that sees nothing is 0 with the log-sum-exp -inf.  Lengths are
  * clamped to [0, S].  The cache and the prefix may be of different types; a 16-bit one has q's.
+ * A value that is not finite (in 8 bits: its scale) makes NaN of the rows that see it, and may of rows up to 384
+ * positions ahead of them, whose weight of 0 it is multiplied by; a key that is not finite, only of rows that see it.
  * Values of 8 bits are weighted in f16 under a power of two of the largest ones (and of no less than the scale
  * 2^-76: values far below that lose bits). */
 typedef struct {

@@ -856,3 +856,23 @@ def test_values_at_the_ends_of_the_range(ops, B, Sq, group, order, fmt):
   check_attention(*ops.attn_prefix(q, prefix, cache, ints(lens), return_lse=True), _attention(q, cache, lens, True, prefix), "prefix")
   plain = make_cache(1, P, 2, torch.bfloat16, 214, torch.bfloat16)  # (values of ordinary size, without scales, ahead of them)
   check_attention(*ops.attn_prefix(q, plain, cache, ints(lens), return_lse=True), _attention(q, cache, lens, True, plain), "16-bit prefix")
+
+
+@pytest.mark.parametrize("fmt", [None] + FORMATS, ids=str)
+@pytest.mark.parametrize("B, S, group", [(1, 1000, 1), (3, 900, 2), (1, 1500, 4)])
+def test_a_whole_prompt_and_its_keys_that_no_row_of_a_block_sees(ops, B, S, group, fmt):
+  # a value that is not finite makes NaN of what sees it, and (with a weight of 0) may of rows of its block of query tiles; rows of the
+  # blocks ahead do not touch it
+  cache = make_cache(B, S, 2, fmt or torch.float16, 220)
+  q = q_of(B, S, 2 * group, torch.float16, 221)
+  clean, lse = ops.attn_cache(q, cache, return_lse=True)
+  check_attention(clean, lse, _attention(q, cache))
+  at = S - 20
+  if fmt is None:
+    cache.v[:, at] = torch.nan
+  else:
+    cache.v_scale[:, :, at] = torch.nan
+  got, got_lse = ops.attn_cache(q, cache, return_lse=True)
+  assert torch.isnan(got[:, at:]).all()
+  ahead = at - 256 // group - 128   # (a block is 256 rows of a key/value head, a tile of keys 128)
+  assert same(got[:, :ahead], clean[:, :ahead]) and same(got_lse, lse)
