@@ -876,3 +876,19 @@ def test_a_whole_prompt_and_its_keys_that_no_row_of_a_block_sees(ops, B, S, grou
   assert torch.isnan(got[:, at:]).all()
   ahead = at - 256 // group - 128   # (a block is 256 rows of a key/value head, a tile of keys 128)
   assert same(got[:, :ahead], clean[:, :ahead]) and same(got_lse, lse)
+
+
+# The 2-norm of an f16 output's error over its own.  A rounding to a step of 2^-10 of values evenly spread over a power of two is off by
+# 2^-10 / sqrt(12) against sqrt(7 / 3): 2^-10 / sqrt(28) = 1.85e-4 in the mean square, and with weights of that error and values that are
+# independent of each other an output's is as large.  So: the weights and the output; where codes times scales are rounded (two query
+# tiles over 8 bits), the values too, and the keys, whose error in a logit is 1.85e-4 |q| |k| of a component each, 1 with normal ones.
+# A fifth more than the root of the sum of squares.
+@pytest.mark.parametrize("fmt", [None] + FORMATS, ids=str)
+@pytest.mark.parametrize("B, Sq, group, tiles", [(1, 1, 4, 0), (50, 1, 4, 0), (3, 2, 8, 0), (8, 20, 2, 1), (3, 100, 1, 1), (2, 100, 2, 2), (1, 300, 2, 2)])
+def test_f16_outputs_are_as_near_as_their_roundings(ops, B, Sq, group, tiles, fmt):
+  cache = make_cache(B, 2000, 2, fmt or torch.float16, 230)
+  q, lens = q_of(B, Sq, 2 * group, torch.float16, 231), [2000 - 17 * i for i in range(B)]
+  got = ops.attn_cache(q, cache, ints(lens)).double()
+  want = _attention(q, cache, lens)[0]
+  roundings = 2 if fmt is None or tiles < 2 else 4
+  assert (got - want).norm() <= 1.2 * (roundings / 28) ** 0.5 * 2.0 ** -10 * want.norm()
