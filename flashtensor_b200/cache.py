@@ -16,7 +16,8 @@ class KVCache:
   head side by side, so that a head is read as one stream.
 
   How many rows of each sequence are filled is the caller's to keep (int32 [B] on the device, one for all
-  layers): ``write`` takes the row to start at, attention and ``read`` the number of rows.
+  layers): ``write`` takes the row to start at, attention and ``read`` the number of rows.  Both are for 8 bits; the
+  rows of a 16-bit cache are the values themselves, to be assigned to (``k[:, a:b] = ...``, ``k.scatter_``).
   """
   __slots__ = ("k", "v", "k_scale", "v_scale")
 

@@ -321,7 +321,10 @@ class PrefixAttn(CacheAttn):
 
 CASES = {"EA": EA, "Attn": Attn, "Gemma2": Gemma2, "SnapKV": SnapKV, "Corm": Corm, "H2O": H2O, "KeyFormer": KeyFormer, "RoCo": RoCo, "SimA": SimA}
 
+# (over a ``KVCache``; not of the reference, whose kernels ``B200Builder`` is asked for)
+CACHE_CASES = {"CacheAttn": CacheAttn, "PrefixAttn": PrefixAttn}
+
 
 def get_model(name="H2O", **kwargs):
   """Factory in the spirit of each reference module's ``get_model()``."""
-  return CASES[name](**kwargs)
+  return (CACHE_CASES if name in CACHE_CASES else CASES)[name](**kwargs)

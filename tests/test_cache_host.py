@@ -161,6 +161,14 @@ def test_cases_keep_their_bookkeeping():
     ft.CacheAttn(3, 8)
 
 
+def test_the_factory_finds_the_cases_over_caches():
+  a, p = ft.get_model("CacheAttn", kv_head_num=2, head_num=8, causal=False), ft.get_model("PrefixAttn", kv_head_num=2, head_num=8)
+  assert type(a) is ft.CacheAttn and not a.causal and type(p) is ft.PrefixAttn and p.head_num == 8
+  assert type(ft.get_model("Attn")) is ft.Attn
+  with pytest.raises(KeyError):
+    ft.get_model("KVCache")
+
+
 def test_structures_match_the_header(tmp_path):
   import os
   import shutil
