@@ -81,9 +81,6 @@ __device__ __forceinline__ void ldsm4_t(uint32_t addr, uint32_t (&r)[4]) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
 }
-__device__ __forceinline__ void lds4(uint32_t addr, uint32_t* r) {
-  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
-}
 __device__ __forceinline__ void prefetch_l2(const void* p) { asm volatile("prefetch.global.L2 [%0];" ::"l"(p)); }
 // x / y, y > 0, in 32 bits where they fit (a 64-bit division takes 0.2 us)
 __device__ __forceinline__ int64_t quotient(int64_t x, int64_t y) {
@@ -790,7 +787,8 @@ cudaError_t launch_stream(const CacheRows* const* c, StreamParams& p, bool bf16,
 //                     128 units 16384 keys 140/135; 256 units 1000 keys 26.6/28.4, 512 units 500 keys 26.7/39.4
 //   16 bits, 16 rows  16 units 8003 keys 25.3/17.2, 128 units 4001 keys 52/43
 //   8 bits, 4 rows    8 units 8000 keys 13.7/15.0; 128 units 4001 keys 30.6/57.8
-//   8 bits, 16 rows   16 units 8003 keys 26/20; 8 units 32000 keys 34/37; 128 units 4001 keys 44/58
+//   8 bits, 16 rows   16 units 8003 keys 26/20; 8 units 32000 keys 34/37 (few units of many keys:
+//                     given up for a rule on their number); 128 units 4001 keys 44/58
 bool streams(const Segment& s, const RowShape& q, int format, int num_sms) {
   if (s.rows > kRows) return false;
   const int64_t units = static_cast<int64_t>(s.N) * q.Hkv;

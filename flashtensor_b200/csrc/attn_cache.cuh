@@ -1,4 +1,4 @@
-// What the kernels of attention over caches share: a segment's rows, partial results, codes, tensor maps.
+// What the kernels of a cache share: pairs of 16-bit values, a segment's rows, partial results, codes, tensor maps.
 #pragma once
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -53,6 +53,9 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
     const __half2 v = __floats2half2_rn(lo, hi);
     return *reinterpret_cast<const uint32_t*>(&v);
   }
+}
+__device__ __forceinline__ void lds4(uint32_t addr, uint32_t* r) {
+  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
 }
 
 // ---- a segment's rows ----------------------------------------------------------------------------

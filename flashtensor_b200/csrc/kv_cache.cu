@@ -15,37 +15,17 @@
 // head, as in a decode step, the heads follow each other.  What is read does not wait for what says whether it counts.
 // On the device: 32 sequences of up to 2001 tokens, 8 heads, to e4m3 (301 MB moved) 66 us = 4.6 TB/s, one token of 16 sequences 1.6 us;
 // 2 sequences of 5003 rows, 8 heads, back to bf16 (60 MB moved) 11.4 us = 5.2 TB/s.
-#include <cuda_bf16.h>
-#include <cuda_fp16.h>
 #include <cuda_fp8.h>
 
-#include "kernels.h"
-#include "sm100_ptx.cuh"
+#include "attn_cache.cuh"
 
 namespace asuka {
-using namespace sm100;
 
 namespace {
 
 constexpr int kRowsPerCta = 32;
 constexpr int kLanes = 8;  // per row
 constexpr int kThreads = kRowsPerCta * kLanes;
-
-template <bool kBF16>
-__device__ __forceinline__ float2 unpack2(uint32_t w) {
-  if constexpr (kBF16) return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&w));
-  else return __half22float2(*reinterpret_cast<const __half2*>(&w));
-}
-template <bool kBF16>
-__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
-  if constexpr (kBF16) {
-    const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
-    return *reinterpret_cast<const uint32_t*>(&v);
-  } else {
-    const __half2 v = __floats2half2_rn(lo, hi);
-    return *reinterpret_cast<const uint32_t*>(&v);
-  }
-}
 
 // Codes of this lane's 16 values (every lane of the row calls it) and the row's scale.
 template <bool kBF16, bool kE4M3>
