@@ -19,6 +19,7 @@
 //     and is merged by attn_merge_kernel in the order of the keys, so results do not depend on which warp was first.
 // Small calls are bound by the launches and by one unit's latency, not by bytes: there a cluster of up to eight CTAs takes a unit, its warps
 // an equal range each, and merges through its distributed shared memory (see `cluster_of`); there is no deal, workspace or second launch.
+// Over 16 bits the weights are rounded to the values' type, as the operands of one product have the same (bf16: 2^-9 on average).
 // Codes of 8 bits go from shared memory straight into matrix fragments:
 //   - codes become f16, exactly (int8 as the low bits of 1024 + 128 + code, less 1152; e4m3 by conversion), and q is brought
 //     to f16 too, a bf16 row times the power of two that puts its largest value in [1, 2): what is lost is below 2^-24 of it;

@@ -24,8 +24,15 @@
 // With f16 output, finer than those roundings together (f16 keys, values and weights: 4.0e-4 to 4.8e-4 of it, the output's own 2.1e-4), and one
 // query tile the f16 tiles are the codes, exactly, and the softmax multiplies logits and weights by the scales in f32 (kExact):
 // 2.8e-4, G4 B32 H40/8 P6001 e4m3 36.9 -> 39.1 us.  bf16 output does not show them (1.7e-3 by itself), and for two query tiles, for which
-// shared memory has no room for the scales as they are, and 4550 clk a pair of steps instead of 2700 in a form that made some, it
-// stays at 3.6e-4 to 5.4e-4.  (Half tiles of codes at a time: 5300 clk.)
+// shared memory has no room for the scales as they are, it stays at 3.6e-4 to 5.4e-4.
+//
+// Over 16 bits the weights have the values' type, since the operands of one product have: with bf16 they are rounded to 2^-9 on average
+// (the error of bf16 output 1.7e-3 -> 2.3e-3), as the prefill's are.
+//
+// Where the time goes, by the clock inside (int8, B2 Sq100 H32/8, 8003 keys: two tiles, 16 key tiles to a CTA; 41 us): set-up 0.7 us, 5.6 until the
+// first S (4.4 of them until the queries are converted and the first codes have come), 30.5 the key tiles, 2.9 the end.  A key tile takes
+// 3750 clk, of which the tensor pipe works for 2050 and the converting warps for 3500: they bound it.  Over 16 bits it takes 2530.  With
+// one query tile of 40 rows it takes 2500 clk over e4m3, of which the converting warps work for 2290.
 #include "attn_cache.cuh"
 
 namespace asuka {
